@@ -48,6 +48,8 @@ EXPORTED_SYMBOLS = (
     "csrspmm_b200_e2m1_quantize_device", "csrspmm_b200_transpose", "csrspmm_b200_transpose_workspace_bytes",
     "csrspmm_b200_spmm_tiled", "csrspmm_b200_tiled_workspace_bytes", "csrspmm_b200_tiled_panel_rows",
     "csrspmm_b200_schedule_create", "csrspmm_b200_schedule_destroy", "csrspmm_b200_schedule_info_get",
+    "csrspmm_b200_route", "csrspmm_b200_route_backward", "csrspmm_b200_sddmm", "csrspmm_b200_distill",
+    "csrspmm_b200_distill_backward", "csrspmm_b200_distill_grad",
 )
 
 
@@ -100,6 +102,20 @@ class PlanInfo(C.Structure):
     """Mirror of ``csrspmm_b200_plan_info``."""
     _fields_ = [("struct_size", C.c_uint32), ("kernel", C.c_int32), ("launches", C.c_int32), ("padded_copy", C.c_int32),
                 ("resident_lanes", C.c_int32), ("row_aligned", C.c_int32)]
+
+
+class RouteArgs(C.Structure):
+    """Mirror of ``csrspmm_b200_route_args``."""
+    _fields_ = [("struct_size", C.c_uint32), ("T", C.c_int32), ("E", C.c_int32), ("k", C.c_int32), ("scores", C.c_void_p),
+                ("ld", C.c_int64), ("score_type", C.c_int32), ("score", C.c_int32), ("bias", C.c_void_p), ("groups", C.c_int32),
+                ("top_groups", C.c_int32), ("group_top", C.c_int32), ("renormalize", C.c_int32), ("scale", C.c_float)]
+
+
+class DistillArgs(C.Structure):
+    """Mirror of ``csrspmm_b200_distill_args``."""
+    _fields_ = [("struct_size", C.c_uint32), ("T", C.c_int32), ("V", C.c_int32), ("logit_type", C.c_int32), ("logits", C.c_void_p),
+                ("ld", C.c_int64), ("nnz", C.c_int64), ("row_ptr", C.c_void_p), ("col_idx", C.c_void_p), ("values", C.c_void_p),
+                ("temperature", C.c_float), ("log_probs", C.c_int32)]
 
 
 class LibraryMissing(RuntimeError):
@@ -200,6 +216,16 @@ def lib() -> C.CDLL:
     L.csrspmm_b200_schedule_destroy.restype = C.c_int
     L.csrspmm_b200_schedule_info_get.argtypes = [C.c_void_p, C.POINTER(ScheduleInfo)]
     L.csrspmm_b200_schedule_info_get.restype = C.c_int
+    L.csrspmm_b200_route.argtypes = [C.POINTER(RouteArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    L.csrspmm_b200_route_backward.argtypes = [C.POINTER(RouteArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                              C.c_void_p]
+    L.csrspmm_b200_sddmm.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+                                     C.c_int64, C.c_float, C.c_void_p, C.c_void_p]
+    L.csrspmm_b200_distill.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p, C.c_void_p]
+    L.csrspmm_b200_distill_backward.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]
+    L.csrspmm_b200_distill_grad.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
+    for name in ("route", "route_backward", "sddmm", "distill", "distill_backward", "distill_grad"):
+        getattr(L, "csrspmm_b200_" + name).restype = C.c_int
     if L.csrspmm_b200_abi_version() != ABI_VERSION:
         raise LibraryMissing(f"{LIB_PATH} has ABI version {L.csrspmm_b200_abi_version()}, expected {ABI_VERSION}")
     _lib = L

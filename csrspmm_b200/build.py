@@ -68,7 +68,7 @@ def build_binding() -> Path:
     """lib/_torch_binding.so: the CPython/torch binding (host code only, links torch, gets the SpMM library's
     functions by address)."""
     LIB_DIR.mkdir(exist_ok=True)
-    newest = max(p.stat().st_mtime for p in (BINDING_SRC, ROOT / "include" / "csrspmm_b200.h"))
+    newest = max(p.stat().st_mtime for p in (BINDING_SRC, BINDING_SRC.parent / "scores.h", ROOT / "include" / "csrspmm_b200.h"))
     if BINDING.exists() and BINDING.stat().st_mtime >= newest:
         return BINDING
     from torch.utils import cpp_extension

@@ -35,6 +35,26 @@ cudaError_t allow_dynamic_smem(size_t bytes)
     return e;
 }
 
+// `cluster`: CTAs of a thread-block cluster, of which `grid` is a multiple.
+template <class... Params, class... Args>
+cudaError_t launch_clusters(void (*kernel)(Params...), unsigned grid, unsigned cluster, unsigned block, size_t smem, cudaStream_t st, Args... args)
+{
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 template <class... Params, class... Args>
 cudaError_t launch_overlapped(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, Args... args)
 {

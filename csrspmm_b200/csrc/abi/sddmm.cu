@@ -1,0 +1,67 @@
+// extern "C" entry point for the gradient of a product for the matrix's stored values (declared in
+// include/csrspmm_b200.h).  No counterpart in the reference.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "../kernels/sddmm_kernel.cuh"
+#include "csrspmm_b200.h"
+#include "pdl.h"
+#include "plan.h"
+
+using namespace csrspmm_b200;
+
+namespace {
+
+template <int L, int NV, int VW, bool LOOP>
+cudaError_t launch(SddmmParams p, cudaStream_t st)
+{
+    constexpr int groups = kSddmmThreads / L;
+    // as many entries for each group of lanes as still give every SM several CTAs, and no more than the row table holds
+    const long long per_group = std::clamp<long long>(p.nnz / ((long long)kSms * 8 * groups), 1, kSddmmMostEntries / groups);
+    p.run = (int)per_group * groups;
+    const unsigned grid = (unsigned)(((long long)p.nnz + p.run - 1) / p.run);
+    return launch_overlapped(sddmm_kernel<L, NV, VW, LOOP>, grid, kSddmmThreads, 0, st, p);
+}
+
+template <int VW>
+cudaError_t launch_width(const SddmmParams& p, cudaStream_t st)
+{
+    if (p.nvec <= 8) return launch<8, 1, VW, false>(p, st);
+    if (p.nvec <= 16) return launch<8, 2, VW, false>(p, st);
+    if (p.nvec <= 32) return launch<8, 4, VW, false>(p, st);
+    if (p.nvec <= 64) return launch<16, 4, VW, false>(p, st);
+    if (p.nvec <= 128) return launch<32, 4, VW, false>(p, st);
+    return launch<32, 4, VW, true>(p, st);
+}
+
+}  // namespace
+
+extern "C" int csrspmm_b200_sddmm(int32_t M, int32_t Kd, int32_t Nd, int64_t nnz, const int32_t* row_ptr, const int32_t* col_idx, const float* G,
+                                  int64_t ldg, const float* B, int64_t ldb, float alpha, float* out, csrspmm_b200_stream_t stream)
+{
+    if (M < 0 || Kd < 0 || Nd < 0 || nnz < 0 || nnz > 0x7fffffffLL || ldg < Nd || ldb < Nd || (nnz > 0 && (M == 0 || Kd == 0)) ||
+        (nnz > 0 && (row_ptr == nullptr || col_idx == nullptr || out == nullptr || (Nd > 0 && (G == nullptr || B == nullptr))))) {
+        set_last_error("sddmm: bad argument");
+        return CSRSPMM_B200_ERR_BAD_ARG;
+    }
+    if (nnz == 0) return CSRSPMM_B200_OK;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const auto on = [&](int floats) {
+        return Nd % floats == 0 && ldg % floats == 0 && ldb % floats == 0 &&
+               ((reinterpret_cast<uintptr_t>(G) | reinterpret_cast<uintptr_t>(B)) & (floats * 4 - 1)) == 0;
+    };
+    SddmmParams p = {};
+    p.M = M, p.Kd = Kd, p.nnz = (int)nnz;
+    p.row_ptr = row_ptr, p.col_idx = col_idx;
+    p.G = G, p.ldg = ldg, p.B = B, p.ldb = ldb, p.alpha = alpha, p.out = out;
+    const int width = on(4) ? 4 : on(2) ? 2 : 1;
+    p.nvec = Nd / width;
+    const cudaError_t e = width == 4 ? launch_width<4>(p, st) : width == 2 ? launch_width<2>(p, st) : launch_width<1>(p, st);
+    if (e != cudaSuccess) {
+        set_last_error("sddmm: launch failed: %s", cudaGetErrorString(e));
+        return CSRSPMM_B200_ERR_CUDA;
+    }
+    return CSRSPMM_B200_OK;
+}

@@ -394,29 +394,34 @@ void expect_args(Py_ssize_t got, Py_ssize_t wanted)
     if (got != wanted) throw std::runtime_error("csrspmm_b200 binding: wrong number of arguments");
 }
 
+template <class Fn>
+void fill(Fn& fn, PyObject* addresses, const char* name)
+{
+    PyObject* o = PyDict_GetItemString(addresses, name);
+    if (o == nullptr) throw std::runtime_error(std::string("csrspmm_b200 binding: no address for ") + name);
+    fn = reinterpret_cast<Fn>(static_cast<uintptr_t>(as_integer(o)));
+}
+void init_scores(PyObject* addresses);
+
 // init(SpmmError, {name: address of csrspmm_b200_<name>})
 PyObject* py_init(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 {
     BEGIN_BINDING
     expect_args(nargs, 2);
-    auto fill = [&](auto& fn, const char* name) {
-        PyObject* o = PyDict_GetItemString(args[1], name);
-        if (o == nullptr) throw std::runtime_error(std::string("csrspmm_b200 binding: no address for ") + name);
-        fn = reinterpret_cast<std::decay_t<decltype(fn)>>(static_cast<uintptr_t>(as_integer(o)));
-    };
-    fill(g_lib.spmm, "spmm");
-    fill(g_lib.spmm_sync, "spmm_sync");
-    fill(g_lib.uses_workspace, "uses_workspace");
-    fill(g_lib.workspace_bytes, "workspace_bytes");
-    fill(g_lib.least_workspace_bytes, "least_workspace_bytes");
-    fill(g_lib.row_stats, "row_stats_device");
-    fill(g_lib.dense2csr_mask_bytes, "dense2csr_mask_bytes");
-    fill(g_lib.dense2csr_count, "dense2csr_count_mask");
-    fill(g_lib.dense2csr_fill, "dense2csr_fill_mask");
-    fill(g_lib.quantize, "e2m1_quantize_device");
-    fill(g_lib.transpose_workspace_bytes, "transpose_workspace_bytes");
-    fill(g_lib.transpose, "transpose");
-    fill(g_lib.check_bounds, "check_bounds_device");
+    fill(g_lib.spmm, args[1], "spmm");
+    fill(g_lib.spmm_sync, args[1], "spmm_sync");
+    fill(g_lib.uses_workspace, args[1], "uses_workspace");
+    fill(g_lib.workspace_bytes, args[1], "workspace_bytes");
+    fill(g_lib.least_workspace_bytes, args[1], "least_workspace_bytes");
+    fill(g_lib.row_stats, args[1], "row_stats_device");
+    fill(g_lib.dense2csr_mask_bytes, args[1], "dense2csr_mask_bytes");
+    fill(g_lib.dense2csr_count, args[1], "dense2csr_count_mask");
+    fill(g_lib.dense2csr_fill, args[1], "dense2csr_fill_mask");
+    fill(g_lib.quantize, args[1], "e2m1_quantize_device");
+    fill(g_lib.transpose_workspace_bytes, args[1], "transpose_workspace_bytes");
+    fill(g_lib.transpose, args[1], "transpose");
+    fill(g_lib.check_bounds, args[1], "check_bounds_device");
+    init_scores(args[1]);
     Py_INCREF(args[0]);
     Py_XSETREF(g_error, args[0]);
     Py_RETURN_NONE;
@@ -808,6 +813,18 @@ void spmm_inplace_marking(const at::Tensor& rp, const at::Tensor& ci, const at::
 
 TORCH_LIBRARY_IMPL(csrspmm_b200, ADInplaceOrView, m) { m.impl("spmm_", spmm_inplace_marking); }
 
+#include "scores.h"
+
+void init_scores(PyObject* addresses)
+{
+    fill(g_scores.route, addresses, "route");
+    fill(g_scores.route_backward, addresses, "route_backward");
+    fill(g_scores.sddmm, addresses, "sddmm");
+    fill(g_scores.distill, addresses, "distill");
+    fill(g_scores.distill_backward, addresses, "distill_backward");
+    fill(g_scores.distill_grad, addresses, "distill_grad");
+}
+
 #define FASTCALL(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL
 PyMethodDef g_methods[] = {
     {"init", FASTCALL(py_init), nullptr},
@@ -818,6 +835,11 @@ PyMethodDef g_methods[] = {
     {"quantize", FASTCALL(py_quantize), nullptr},
     {"transpose", FASTCALL(py_transpose), nullptr},
     {"matmul", FASTCALL(py_matmul), nullptr},
+    {"route", FASTCALL(py_route), nullptr},
+    {"sddmm", FASTCALL(py_sddmm), nullptr},
+    {"weighted_spmm", FASTCALL(py_weighted_spmm), nullptr},
+    {"distill_loss", FASTCALL(py_distill_loss), nullptr},
+    {"distill_loss_grad", FASTCALL(py_distill_loss_grad), nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -446,3 +446,69 @@ def csr2dense(row_ptr: torch.Tensor, col_idx: torch.Tensor, values: torch.Tensor
         _lib.check(_lib.lib().csrspmm_b200_csr2dense(H, W, row_ptr.data_ptr(), col_idx.data_ptr(), values.data_ptr(),
                                                      out.data_ptr(), max(W, 1), stream), "csrspmm_b200_csr2dense")
     return out
+
+
+# ---- sparse rows of scores: routing, the gradient for stored values, distillation ------------------------------
+
+def _with_autograd():
+    """The operators' schemas, without which a call that wants a gradient has nowhere to go."""
+    from . import torch_library  # noqa: F401  (it imports this module)
+
+
+def route(logits: torch.Tensor, k: int, *, bias: torch.Tensor | None = None, score: str = "softmax", groups: int = 1,
+          top_groups: int = 1, group_top: int = 1, renormalize: bool = True, scale: float = 1.0):
+    """The CSR matrix tokens x experts of a router: (row_ptr, col_idx, values) from ``logits`` (T x E; float32, float16 or
+    bfloat16, any strides), ``k`` entries a row with ascending columns.
+
+    Scores are ``softmax`` or ``sigmoid`` of the logits; ``bias`` (E, float32) is added for the choice only.  With
+    ``top_groups < groups`` the experts form ``groups`` runs, of which the ``top_groups`` best by the sum of their ``group_top`` (1 or 2)
+    best experts are open to a token.  Ties go to the lower index, and the choice is the one that exact arithmetic makes.  Values are the
+    chosen scores, divided by their sum with ``renormalize``, times ``scale`` (float32).  A logit of -inf is an expert that is not
+    available: it ranks behind all others of the open groups and weighs 0, so that a row with nothing available has k zeros.  A NaN
+    (softmax: or +inf) makes its row's values NaN; the columns stay distinct and inside the matrix.  Experts up to 1024, k and groups
+    up to 32.
+
+    ``values`` is differentiable in ``logits`` (the first derivative; the choice has none, nor has ``bias``).  ``transpose_csr`` of the result lists
+    each expert's tokens; ``weighted_spmm`` adds up what the experts answered.
+    """
+    if logits.requires_grad:
+        _with_autograd()
+    return _lib.binding().route(logits, k, bias, score, groups, top_groups, group_top, renormalize, scale)
+
+
+def sddmm(row_ptr: torch.Tensor, col_idx: torch.Tensor, G: torch.Tensor, B: torch.Tensor, alpha: float = 1.0) -> torch.Tensor:
+    """``alpha * <G[row(e)], B[col(e)]>`` for every entry e of a CSR pattern (float32): a dense product sampled at the pattern, which is
+    the gradient of ``alpha * A @ B`` for A's values when G is that of the product.  Not differentiable itself (``weighted_spmm`` is)."""
+    return _lib.binding().sddmm(row_ptr, col_idx, G, B, alpha)
+
+
+def weighted_spmm(row_ptr: torch.Tensor, col_idx: torch.Tensor, values: torch.Tensor, B: torch.Tensor, alpha: float = 1.0) -> torch.Tensor:
+    """``alpha * A @ B`` as a new tensor, differentiable in A's ``values`` and in ``B`` (the first derivative): for matrices whose entries are
+    learnt, such as a router's weights.  ``torch.ops.csrspmm_b200.spmm`` is the product without a gradient for the values."""
+    if values.requires_grad or B.requires_grad:
+        _with_autograd()
+    return _lib.binding().weighted_spmm(row_ptr, col_idx, values, B, alpha)
+
+
+def distill_loss(logits: torch.Tensor, row_ptr: torch.Tensor, col_idx: torch.Tensor, values: torch.Tensor, *, temperature: float = 1.0,
+                 log_probs: bool = False) -> torch.Tensor:
+    """Per row the divergence of a student from a teacher of whom some logits are known (a CSR matrix T x V, float32 values, any order):
+    ``t^2 * sum p (ln p - ln q)`` over the row's entries, with ``q = softmax(logits / t)`` and ``p = softmax(values / t)`` over the entries.  With
+    ``log_probs`` the values are log-probabilities at that temperature and ``p = exp(values)`` as they are, so that their sum may be below 1.
+
+    ``logits`` (T x V) are float32, float16 or bfloat16; the losses (T) are float32 and differentiable in ``logits`` (the first derivative; the
+    teacher has none).  A row without entries, or whose entries weigh nothing, is left out: loss 0, gradient 0.
+    """
+    if logits.requires_grad:
+        _with_autograd()
+    return _lib.binding().distill_loss(logits, row_ptr, col_idx, values, temperature, log_probs)
+
+
+def distill_loss_grad(logits: torch.Tensor, row_ptr: torch.Tensor, col_idx: torch.Tensor, values: torch.Tensor,
+                      weight: torch.Tensor | float = 1.0, *, temperature: float = 1.0, log_probs: bool = False):
+    """``distill_loss`` and the gradient of ``sum(weight * loss)`` for the logits, in one launch that takes the logits from memory once:
+    ``(loss, dlogits)``.  ``weight`` (float32, one per row, or a number) is what the caller's reduction gives each row, 1 / T for
+    a mean.  Nothing is recorded for autograd: hand the gradient on with ``logits.backward(dlogits)``."""
+    if not isinstance(weight, torch.Tensor):
+        weight = torch.full((), float(weight), dtype=torch.float32, device=logits.device)
+    return _lib.binding().distill_loss_grad(logits, row_ptr, col_idx, values, weight, temperature, log_probs)

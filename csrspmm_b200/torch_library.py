@@ -51,6 +51,23 @@ _library.define("spmm_(Tensor row_ptr, Tensor col_idx, Tensor values, Tensor B, 
                 "str kernel) -> ()", tags=(torch.Tag.pt2_compliant_tag,))
 _library.define("transpose(Tensor row_ptr, Tensor col_idx, Tensor values, SymInt Kd) -> (Tensor, Tensor, Tensor)",
                 tags=(torch.Tag.pt2_compliant_tag,))
+# Routing, the gradient for a matrix's stored values, distillation (csrc/torch/scores.h).  route, weighted_spmm and distill_loss
+# have gradients; *_backward and distill_with_stats are what those are made of.
+_library.define("route(Tensor logits, int k, Tensor? bias, str score, int groups, int top_groups, int group_top, bool renormalize, float scale) "
+                "-> (Tensor, Tensor, Tensor)", tags=(torch.Tag.pt2_compliant_tag,))
+_library.define("route_backward(Tensor grad, Tensor logits, Tensor col_idx, Tensor values, int k, str score, bool renormalize, float scale) "
+                "-> Tensor", tags=(torch.Tag.pt2_compliant_tag,))
+_library.define("sddmm(Tensor row_ptr, Tensor col_idx, Tensor G, Tensor B, float alpha) -> Tensor", tags=(torch.Tag.pt2_compliant_tag,))
+_library.define("weighted_spmm(Tensor row_ptr, Tensor col_idx, Tensor values, Tensor B, float alpha) -> Tensor",
+                tags=(torch.Tag.pt2_compliant_tag,))
+_library.define("distill_loss(Tensor logits, Tensor row_ptr, Tensor col_idx, Tensor values, float temperature, bool log_probs) -> Tensor",
+                tags=(torch.Tag.pt2_compliant_tag,))
+_library.define("distill_with_stats(Tensor logits, Tensor row_ptr, Tensor col_idx, Tensor values, float temperature, bool log_probs) "
+                "-> (Tensor, Tensor)", tags=(torch.Tag.pt2_compliant_tag,))
+_library.define("distill_backward(Tensor grad, Tensor logits, Tensor row_ptr, Tensor col_idx, Tensor values, Tensor stats, float temperature, "
+                "bool log_probs) -> Tensor", tags=(torch.Tag.pt2_compliant_tag,))
+_library.define("distill_loss_grad(Tensor logits, Tensor row_ptr, Tensor col_idx, Tensor values, Tensor weight, float temperature, "
+                "bool log_probs) -> (Tensor, Tensor)", tags=(torch.Tag.pt2_compliant_tag,))
 
 
 @torch.library.register_fake("csrspmm_b200::spmm")
@@ -66,6 +83,49 @@ def _spmm_inplace_fake(row_ptr, col_idx, values, B, C, alpha, beta, kernel):
 @torch.library.register_fake("csrspmm_b200::transpose")
 def _transpose_fake(row_ptr, col_idx, values, Kd):
     return row_ptr.new_empty((Kd + 1,)), torch.empty_like(col_idx), torch.empty_like(values)
+
+
+@torch.library.register_fake("csrspmm_b200::route")
+def _route_fake(logits, k, bias, score, groups, top_groups, group_top, renormalize, scale):
+    T = logits.shape[0]
+    return (logits.new_empty((T + 1,), dtype=torch.int32), logits.new_empty((T * k,), dtype=torch.int32),
+            logits.new_empty((T * k,), dtype=torch.float32))
+
+
+@torch.library.register_fake("csrspmm_b200::route_backward")
+def _route_backward_fake(grad, logits, col_idx, values, k, score, renormalize, scale):
+    return logits.new_empty(logits.shape)
+
+
+@torch.library.register_fake("csrspmm_b200::sddmm")
+def _sddmm_fake(row_ptr, col_idx, G, B, alpha):
+    return G.new_empty(col_idx.shape)
+
+
+@torch.library.register_fake("csrspmm_b200::weighted_spmm")
+def _weighted_spmm_fake(row_ptr, col_idx, values, B, alpha):
+    return B.new_empty((row_ptr.shape[0] - 1, B.shape[1]))
+
+
+@torch.library.register_fake("csrspmm_b200::distill_loss")
+def _distill_loss_fake(logits, row_ptr, col_idx, values, temperature, log_probs):
+    return logits.new_empty((logits.shape[0],), dtype=torch.float32)
+
+
+@torch.library.register_fake("csrspmm_b200::distill_with_stats")
+def _distill_with_stats_fake(logits, row_ptr, col_idx, values, temperature, log_probs):
+    T = logits.shape[0]
+    return logits.new_empty((T,), dtype=torch.float32), logits.new_empty((4 * T,), dtype=torch.float32)
+
+
+@torch.library.register_fake("csrspmm_b200::distill_backward")
+def _distill_backward_fake(grad, logits, row_ptr, col_idx, values, stats, temperature, log_probs):
+    return logits.new_empty(logits.shape)
+
+
+@torch.library.register_fake("csrspmm_b200::distill_loss_grad")
+def _distill_loss_grad_fake(logits, row_ptr, col_idx, values, weight, temperature, log_probs):
+    return logits.new_empty((logits.shape[0],), dtype=torch.float32), logits.new_empty(logits.shape)
 
 
 try:

@@ -350,6 +350,80 @@ int csrspmm_b200_transpose(int32_t M, int32_t Kd, int64_t nnz, const int32_t* ro
                            const float* values, int32_t* t_row_ptr, int32_t* t_col_idx, float* t_values, void* workspace,
                            size_t workspace_bytes, csrspmm_b200_stream_t stream);
 
+/* ---- routing: dense scores -> CSR by rank (new) ----------------------------------------------
+ * The CSR matrix (T x E) of the k experts that each of T tokens is sent to, from a row of E scores x a token:
+ *     s = softmax(x) or sigmoid(x);  c = s + bias (for the choice only; bias may be NULL)
+ *     the experts form `groups` runs of E / groups; a group counts as the sum of its group_top (1 or 2) largest c, and the
+ *     k largest c of the top_groups best groups are taken (ties: the lower index), as exact arithmetic would
+ *     value = scale * s / (sum of the s taken)  with renormalize, else scale * s
+ * Rows hold exactly k entries with ascending columns.  An x of -infinity is an expert that is not available: it is
+ * ranked behind all others of the groups taken and its value is 0; where nothing is available all k values are 0.  A row with a
+ * NaN (softmax: or +infinity) has distinct columns inside the matrix and values of NaN.
+ * Scores are device memory, fp32, fp16 or bf16, `ld` elements from row to row; everything is computed in fp32, and in 64 bits where
+ * two choices are nearer than that tells apart.  E at most 1024, k and groups at most 32. */
+#define CSRSPMM_B200_F32 0
+#define CSRSPMM_B200_F16 1
+#define CSRSPMM_B200_BF16 2
+#define CSRSPMM_B200_SOFTMAX 0
+#define CSRSPMM_B200_SIGMOID 1
+typedef struct csrspmm_b200_route_args {
+    uint32_t struct_size; /* sizeof(csrspmm_b200_route_args), checked */
+    int32_t T, E, k;
+    const void* scores;   /* T rows of E */
+    int64_t ld;
+    int32_t score_type;   /* CSRSPMM_B200_F32, _F16 or _BF16 */
+    int32_t score;        /* CSRSPMM_B200_SOFTMAX or _SIGMOID */
+    const float* bias;    /* E, or NULL */
+    int32_t groups, top_groups, group_top; /* 1, 1, 1: no groups */
+    int32_t renormalize;
+    float scale;
+} csrspmm_b200_route_args;
+/* row_ptr T + 1, col_idx and values T * k.  Asynchronous. */
+int csrspmm_b200_route(const csrspmm_b200_route_args* args, int32_t* row_ptr, int32_t* col_idx, float* values, csrspmm_b200_stream_t stream);
+/* The gradient of the scores (T rows of E in their type, ldd apart, every element written) from that of the values; col_idx and values
+ * as csrspmm_b200_route gave them, dvalues_stride elements from one gradient to the next (0: one for all).  The choice and the
+ * bias have none.  Asynchronous. */
+int csrspmm_b200_route_backward(const csrspmm_b200_route_args* args, const int32_t* col_idx, const float* values, const float* dvalues,
+                                int64_t dvalues_stride, void* dscores, int64_t ldd, csrspmm_b200_stream_t stream);
+
+/* ---- the gradient for the stored values (new) --------------------------------------------------
+ * out[e] = alpha * <G[row(e), :], B[col(e), :]> for the nnz entries of a CSR pattern: the gradient of C = alpha * A * B for A's
+ * values, where G (M x Nd, ldg) is that of C.  Device pointers, asynchronous.  A column outside [0, Kd) counts as the nearest one inside,
+ * as in a product. */
+int csrspmm_b200_sddmm(int32_t M, int32_t Kd, int32_t Nd, int64_t nnz, const int32_t* row_ptr, const int32_t* col_idx, const float* G,
+                       int64_t ldg, const float* B, int64_t ldb, float alpha, float* out, csrspmm_b200_stream_t stream);
+
+/* ---- distillation: a CSR matrix of a teacher's entries against dense logits (new) --------------
+ * Per row, with z = logits / t, q = softmax(z), p = softmax(values / t) over the row's entries (log_probs: p = exp(values), taken as they
+ * are) and P = sum p:
+ *     loss = t^2 * sum_i p_i (ln p_i - z[col_i] + logsumexp z)
+ *     dlogits_j = weight * t * (P q_j - sum of the p_i with col_i = j)
+ * A row without entries, or with none that weighs anything, has loss 0 and gradient 0 whatever its logits hold.  Entries may come in any
+ * order; a column named twice counts with both.  A column outside [0, V) counts as the nearest one inside.
+ * Logits are fp32, fp16 or bf16, computed with in fp32. */
+typedef struct csrspmm_b200_distill_args {
+    uint32_t struct_size; /* sizeof(csrspmm_b200_distill_args), checked */
+    int32_t T, V;
+    int32_t logit_type;   /* CSRSPMM_B200_F32, _F16 or _BF16 */
+    const void* logits;   /* T rows of V, device memory */
+    int64_t ld;           /* elements from row to row */
+    int64_t nnz;
+    const int32_t* row_ptr;
+    const int32_t* col_idx;
+    const float* values;
+    float temperature;    /* t: positive and finite */
+    int32_t log_probs;
+} csrspmm_b200_distill_args;
+/* loss: T floats.  stats (16-byte aligned, 4 * T floats): what _distill_backward needs, or NULL.  Asynchronous. */
+int csrspmm_b200_distill(const csrspmm_b200_distill_args* args, float* loss, float* stats, csrspmm_b200_stream_t stream);
+/* dlogits (T rows of V in the logits' type, ldd apart, not in the logits' place) from the stats of the same arguments; weight_stride
+ * elements from one row's weight to the next (0: one for all).  Asynchronous. */
+int csrspmm_b200_distill_backward(const csrspmm_b200_distill_args* args, const float* stats, const float* weight, int64_t weight_stride,
+                                  void* dlogits, int64_t ldd, csrspmm_b200_stream_t stream);
+/* Loss and dlogits in one launch that takes the logits from memory once. */
+int csrspmm_b200_distill_grad(const csrspmm_b200_distill_args* args, const float* weight, int64_t weight_stride, float* loss, void* dlogits,
+                              int64_t ldd, csrspmm_b200_stream_t stream);
+
 /* ---- multi-GPU row partition (new) ------------------------------------------------------------
  * Contiguous row blocks [bounds[g], bounds[g+1]) for g < parts with near-equal cost, where the
  * cost of a row is its nnz + row_weight (row_weight = 1 balances B-row reads against C-row
