@@ -53,31 +53,77 @@ cudaError_t for_type(int type, F&& f)
     return f(__nv_bfloat16());
 }
 
-// Small CTAs for short rows: four warps read 2048 columns of 2 bytes in one go.
-constexpr int kFew = 128, kMany = 512;
-bool short_rows(const csrspmm_b200_distill_args* a, int parts) { return a->V / parts <= 8192; }
+int element_size(int type) { return type == CSRSPMM_B200_F32 ? 4 : 2; }
 
-// CTAs of a row: enough that the chip has two per SM, as long as each has a few thousand columns.
-int row_parts(const csrspmm_b200_distill_args* a, int most)
+// Cuts the rows into `parts`, a power of two; returns the CTAs of T rows.
+unsigned cut(const csrspmm_b200_distill_args* a, long long parts, DistillParams* p)
 {
-    int parts = 1;
-    while (parts < most && (long long)a->T * parts < 2 * kSms && a->V / (2 * parts) >= 4096) parts *= 2;
-    return parts;
+    for (p->log_parts = 0; 1LL << p->log_parts < parts;) ++p->log_parts;
+    p->per = (int)((a->V + parts - 1) / parts + 63) / 64 * 64;
+    return (unsigned)(a->T * parts);
+}
+
+// Rows that are few are cut further, down to some thousand columns a part, until every SM has two CTAs.
+bool too_few(const csrspmm_b200_distill_args* a, long long parts) { return a->T * parts < 2 * kSms && a->V / (2 * parts) >= 2048; }
+
+cudaError_t launch_gradient(const csrspmm_b200_distill_args* a, DistillParams p, cudaStream_t st)
+{
+    // vectors that a CTA of each shape holds
+    constexpr int kSmall = 128 * 2, kMiddle = 128 * 8, kLarge = 256 * 8;
+    const int per_vector = 16 / element_size(a->logit_type);
+    long long parts = 1;
+    while (a->V > parts * kLarge * per_vector || too_few(a, parts)) parts *= 2;  // parts are rounded to 64 columns, which divide kLarge vectors
+    const unsigned grid = cut(a, parts, &p);
+    const int vectors = p.per / per_vector;
+    return for_type(a->logit_type, [&](auto zero) {
+        using T = decltype(zero);
+        if (vectors <= kSmall) return launch_overlapped(distill_gradient_kernel<T, 128, 2>, grid, 128, 0, st, p);
+        if (vectors <= kMiddle) return launch_overlapped(distill_gradient_kernel<T, 128, 8>, grid, 128, 0, st, p);
+        return launch_overlapped(distill_gradient_kernel<T, 256, 8>, grid, 256, 0, st, p);
+    });
+}
+
+constexpr int kPartBytes = 65536;         // of a part, as far as clusters go: three CTAs of one slot fit an SM
+constexpr int kDynamicSmem = 216 * 1024;  // of a CTA, beside RingShared
+
+// The ring kernel's manager walks a row's entries with one warp; where rows have more than this many, all warps of the long kernel do.
+constexpr int kMostEntries = 2048;
+
+template <class T, int WORKERS, bool GRADIENT>
+cudaError_t launch_ring(const csrspmm_b200_distill_args* a, DistillParams p, int ctas_per_sm, cudaStream_t st)
+{
+    constexpr auto kernel = distill_ring_kernel<T, WORKERS, GRADIENT>;
+    const int parts = 1 << p.log_parts;
+    // A few waves of clusters, so that the SMs end together, of two to four rows each where there are as many.
+    p.rows = (int)std::clamp<long long>(((long long)a->T * parts) / ((long long)kSms * ctas_per_sm * 3), 1, WORKERS <= 128 ? 4 : 2);
+    p.slots = WORKERS <= 128 ? std::min(p.rows, 2) : 1;
+    const size_t smem = (size_t)p.ring_offset + (size_t)p.slots * p.slot_bytes;
+    const cudaError_t e = allow_dynamic_smem<kernel>(smem);
+    if (e != cudaSuccess) return e;
+    const unsigned clusters = (unsigned)(((long long)a->T + p.rows - 1) / p.rows);
+    return launch_clusters(kernel, clusters * (unsigned)parts, (unsigned)parts, WORKERS + 32, smem, st, p);
 }
 
 template <bool GRADIENT>
-cudaError_t launch_loss(const csrspmm_b200_distill_args* a, const DistillParams& p, cudaStream_t st)
+cudaError_t launch_loss(const csrspmm_b200_distill_args* a, DistillParams p, cudaStream_t st)
 {
-    const int parts = row_parts(a, kDistillMostCtas);
-    const unsigned grid = (unsigned)(a->T * (long long)parts);
+    const int size = element_size(a->logit_type);
+    long long parts = 1;
+    while (parts < kDistillMostCtas && ((long long)a->V * size > parts * kPartBytes || too_few(a, parts))) parts *= 2;
+    const unsigned grid = cut(a, parts, &p);
+    const long long slot = (long long)p.per * size, before = GRADIENT ? ((long long)p.per / 32 + 1 + 31) / 32 * 128 : 0;
+    if (before + slot > kDynamicSmem || a->nnz / std::max(a->T, 1) > kMostEntries)
+        return for_type(a->logit_type, [&](auto zero) {
+            return launch_clusters(distill_long_kernel<decltype(zero), GRADIENT>, grid, (unsigned)parts, kLongThreads, 0, st, p);
+        });
+    p.slot_bytes = (int)slot;
+    p.ring_offset = (int)before;
     return for_type(a->logit_type, [&](auto zero) {
         using T = decltype(zero);
-        if (parts > 1) {
-            if (short_rows(a, parts)) return launch_clusters(distill_kernel<T, kFew, GRADIENT, true>, grid, parts, kFew, 0, st, p);
-            return launch_clusters(distill_kernel<T, kMany, GRADIENT, true>, grid, parts, kMany, 0, st, p);
-        }
-        if (short_rows(a, 1)) return launch_overlapped(distill_kernel<T, kFew, GRADIENT, false>, grid, kFew, 0, st, p);
-        return launch_overlapped(distill_kernel<T, kMany, GRADIENT, false>, grid, kMany, 0, st, p);
+        if (p.slot_bytes <= 4096) return launch_ring<T, 32, GRADIENT>(a, p, 14, st);
+        if (p.slot_bytes <= 8192) return launch_ring<T, 128, GRADIENT>(a, p, 6, st);
+        if (p.slot_bytes <= kPartBytes) return launch_ring<T, 256, GRADIENT>(a, p, 3, st);
+        return launch_ring<T, 512, GRADIENT>(a, p, 1, st);
     });
 }
 
@@ -113,14 +159,7 @@ int csrspmm_b200_distill_backward(const csrspmm_b200_distill_args* a, const floa
     DistillParams p = params(a);
     p.stats = const_cast<float4*>(reinterpret_cast<const float4*>(stats));
     p.weight = weight, p.weight_stride = weight_stride, p.dx = dlogits, p.ldd = ldd;
-    const int parts = (int)std::max<long long>(1, std::min<long long>(a->V / 4096, std::max<long long>(a->V / 32768, 4LL * kSms / a->T)));
-    const unsigned grid = (unsigned)(a->T * (long long)parts);
-    return finish(for_type(a->logit_type, [&](auto zero) {
-        using T = decltype(zero);
-        cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-        if (short_rows(a, parts)) return launch_overlapped(distill_backward_kernel<T, kFew>, grid, kFew, 0, st, p, parts);
-        return launch_overlapped(distill_backward_kernel<T, kMany>, grid, kMany, 0, st, p, parts);
-    }));
+    return finish(launch_gradient(a, p, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 int csrspmm_b200_distill_grad(const csrspmm_b200_distill_args* a, const float* weight, int64_t weight_stride, float* loss, void* dlogits, int64_t ldd,

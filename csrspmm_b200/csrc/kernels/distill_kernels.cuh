@@ -6,17 +6,24 @@
 //
 // No counterpart in the reference, whose CSR matrices are only multiplied (src/csrspmm.cpp:28-75).
 //
-// A row of logits belongs to one CTA, or to a cluster of up to eight where there are too few rows to fill the chip: each takes
-// a run of columns, and the running maximum and sum of exp(z - max) of the parts meet in distributed shared memory.  The entries of
-// the teacher are few and are read by every CTA of the row.
+// Loss, and loss with gradient (distill_ring_kernel): a row of logits belongs to a CTA or to a cluster of up to eight, each of which takes a
+// run of columns.  Bulk copies bring the run into shared memory and the runs of the next rows behind it, so that memory is never waited for row by
+// row; from there it is read for the maximum, for the sum and for the gradient, and memory gives each row once.  What
+// the parts found meets in distributed shared memory.  The teacher's entries are few: one warp makes their shares.
+// The gradient alone (distill_gradient_kernel) needs no sum: every thread holds up to eight vectors.  Rows that are longer than a
+// cluster's shared memory are read twice (distill_long_kernel).
 //
-// Sums, maxima and the loss are fp32; everything is taken relative to the row's maximum, so that neither values of the type's
-// lowest nor infinities in masked columns meet a product: exp((x - m) c) is 0 there.
+// Sums, maxima and the loss are fp32.  Exponentials are 2^y with y = x c - m c, c = log2(e) / t, m a maximum: one fused multiply-add each.  The
+// product m c is rounded once and the same rounded one serves the sum, the loss and the gradient, so that its rounding cancels.  Where m c
+// overflows (a row of the type's lowest) y = (x - m) c.
 #pragma once
 
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
+#include <type_traits>
+
+#include "async_copy.cuh"
 #include "common.cuh"
 #include "score_types.cuh"
 
@@ -35,11 +42,14 @@ struct DistillParams {
     float temperature, inv_t;
     int log_probs;
     float* loss;
-    float4* stats;        // per row: max x, sum exp(z - max z), max v, sum exp((v - max v) / t)  (log_probs: 0, 1)
+    float4* stats;        // per row: max x, sum exp(z - max z), max v, sum exp((v - max v) / t)  (log_probs: 0, sum exp v)
     const float* weight;  // per row, g above
     long long weight_stride;
     void* dx;
     long long ldd;
+    int log_parts, per;  // a row is cut into 2^log_parts runs of `per` columns, a multiple of 64
+    // the ring kernel's: rows of a CTA or cluster, copies on their way and the room of each, the shared memory before them
+    int rows, slots, slot_bytes, ring_offset;
 };
 
 __device__ __forceinline__ float exp2_approx(float v)
@@ -49,328 +59,846 @@ __device__ __forceinline__ float exp2_approx(float v)
     return r;
 }
 
-// A maximum and a sum of exponentials relative to it
+__device__ __forceinline__ Pair exp2_approx(Pair v)
+{
+    const float2 w = halves(v);
+    return pair_of(exp2_approx(w.x), exp2_approx(w.y));
+}
+
+// y above, for one maximum
+struct Exponent {
+    float m, mc, c;
+    bool far;
+    __device__ __forceinline__ Exponent(float top, float scale)
+    {
+        m = top;
+        c = scale;
+        mc = __fmul_rn(top, scale);
+        far = !(fabsf(mc) <= -kLowest);
+    }
+    template <bool FAR>
+    __device__ __forceinline__ float of(float x) const
+    {
+        return FAR ? (x - m) * c : __fmaf_rn(x, c, -mc);
+    }
+    __device__ __forceinline__ float of(float x) const { return far ? of<true>(x) : of<false>(x); }
+    template <bool FAR>
+    __device__ __forceinline__ Pair of(Pair x) const
+    {
+        if constexpr (FAR) {
+            const float2 v = halves(x);
+            return pair_of(of<true>(v.x), of<true>(v.y));
+        } else {
+            return fma2(x, pair_of(c, c), pair_of(-mc, -mc));
+        }
+    }
+    // of a smaller maximum, whose own product was rounded too
+    __device__ __forceinline__ float of_max(float other) const { return far ? (other - m) * c : __fsub_rn(__fmul_rn(other, c), mc); }
+};
+
+// A maximum and the sum of 2^y relative to it; none: kLowest and 0.
 struct MaxSum {
     float m, s;
 };
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c)
-{
-    const float m = fmaxf(a.m, b.m);
-    return {m, a.s * exp2_approx((a.m - m) * c) + b.s * exp2_approx((b.m - m) * c)};
-}
-
-// What a thread sees of a row's part [c0, c1): whole 16-byte vectors from the first aligned element on, the rest one by one.
+// What a thread sees of a row's part [c0, c1): whole 16-byte vectors from the first aligned element on; of the at most
+// 2 (N - 1) elements before and behind, one a thread.
 template <class T>
 struct Part {
     static constexpr int N = 16 / (int)sizeof(T);
-    int head, vectors, tail0;  // elements [c0, c0 + head), then `vectors` vectors, then [tail0, c1)
+    int first, vectors, edge;  // the first vector's column; this thread's single element, or -1
     __device__ __forceinline__ Part(const T* row, int c0, int c1)
     {
         const int off = (int)((reinterpret_cast<uintptr_t>(row + c0) & 15u) / sizeof(T));
-        head = min(off ? N - off : 0, c1 - c0);
-        vectors = (c1 - c0 - head) / N;
-        tail0 = c0 + head + vectors * N;
+        const int head = min(off ? N - off : 0, c1 - c0);
+        first = c0 + head;
+        vectors = (c1 - first) / N;
+        const int behind = first + vectors * N, tid = (int)threadIdx.x;
+        edge = tid < head ? c0 + tid : behind + (tid - head) < c1 ? behind + (tid - head) : -1;
     }
 };
 
-template <int THREADS>
-struct BlockSums {
-    float v[THREADS / 32];
+// The row and the columns that a CTA takes.
+struct Place {
+    int row, rank, c0, c1;
+    __device__ __forceinline__ explicit Place(const DistillParams& p) : Place(p, (int)(blockIdx.x >> p.log_parts)) {}
+    __device__ __forceinline__ Place(const DistillParams& p, int r)
+    {
+        row = r;
+        rank = (int)blockIdx.x & ((1 << p.log_parts) - 1);
+        c0 = (int)min((long long)rank * p.per, (long long)p.V);
+        c1 = (int)min((long long)c0 + p.per, (long long)p.V);
+    }
 };
-
-// The sum over the block, in every thread; `room` is free again after the next barrier.
-template <int THREADS>
-__device__ __forceinline__ float block_sum(float v, BlockSums<THREADS>& room)
-{
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) room.v[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) sum += room.v[w];
-    return sum;
-}
-template <int THREADS>
-__device__ __forceinline__ float block_max(float v, BlockSums<THREADS>& room)
-{
-    v = warp_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) room.v[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float m = room.v[0];
-#pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) m = fmaxf(m, room.v[w]);
-    return m;
-}
 
 // The teacher's entries of a row
 struct Teacher {
-    int begin, count;
+    int count;
     const int* cols;
     const float* v;
     float top, sum;  // p = exp((v - top) / t) / sum
 
-    __device__ __forceinline__ float share(const DistillParams& p, int i) const
+    __device__ __forceinline__ float share(const DistillParams& p, float at) const
     {
-        const float at = __ldg(v + i);
         if (p.log_probs) return expf(at);
         return at > -CUDART_INF_F ? expf((at - top) * p.inv_t) / sum : at != at ? at : 0.0f;
     }
     __device__ __forceinline__ int column(const DistillParams& p, int i) const { return min(max(__ldg(cols + i), 0), p.V - 1); }
 };
 
-__device__ __forceinline__ Teacher teacher_of(const DistillParams& p, int row)
+__device__ __forceinline__ Teacher teacher_of(const DistillParams& p, int from, int to)  // its two row offsets
 {
     Teacher t;
-    t.begin = min(max(__ldg(p.row_ptr + row), 0), p.nnz);
-    t.count = max(min(__ldg(p.row_ptr + row + 1), p.nnz) - t.begin, 0);
-    t.cols = p.col_idx + t.begin;
-    t.v = p.values + t.begin;
+    const int begin = min(max(from, 0), p.nnz);
+    t.count = max(min(to, p.nnz) - begin, 0);
+    t.cols = p.col_idx + begin;
+    t.v = p.values + begin;
     t.top = 0.0f;
     t.sum = 1.0f;
     return t;
 }
 
-// The columns a CTA of the row takes.
-__device__ __forceinline__ void part_bounds(int V, int part, int parts, int* c0, int* c1)
+// An entry, and the student's logit in its column
+struct Entry {
+    float v, x;
+    int col;
+};
+
+// A thread's entries: the first is asked for at once and used late.
+template <class T, int THREADS>
+struct Entries {
+    const DistillParams& p;
+    const Teacher& t;
+    const T* row;
+    Entry first = {};
+    __device__ __forceinline__ Entries(const DistillParams& params, const Teacher& teacher, const T* x) : p(params), t(teacher), row(x)
+    {
+        if ((int)threadIdx.x < t.count) first = load(threadIdx.x);
+    }
+    __device__ __forceinline__ Entry load(int i) const
+    {
+        Entry e;
+        e.col = t.column(p, i);
+        e.v = __ldg(t.v + i);
+        e.x = to_f32(row[e.col]);
+        return e;
+    }
+    template <class F>
+    __device__ __forceinline__ void each(F&& f) const
+    {
+        if ((int)threadIdx.x < t.count) f((int)threadIdx.x, first);
+        for (int i = threadIdx.x + THREADS; i < t.count; i += THREADS) f(i, load(i));
+    }
+};
+
+// What the warps of a CTA hand one another
+template <int THREADS>
+struct Room {
+    MaxSum part[THREADS / 32];
+    float top[THREADS / 32], sum[THREADS / 32], cross[THREADS / 32];
+    MaxSum block;
+};
+
+// The maximum and sum of N lanes' (a power of two), each its own: the largest maximum first, then every sum is brought to it once.
+template <int N>
+__device__ __forceinline__ MaxSum join_lanes(MaxSum mine, float c)
 {
-    const int per = ((V + parts - 1) / parts + 63) / 64 * 64;
-    *c0 = (int)min((long long)part * per, (long long)V);
-    *c1 = (int)min((long long)*c0 + per, (long long)V);
+    float m = mine.m;
+#pragma unroll
+    for (int d = N / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kAllLanes, m, d));
+    float s = mine.s * exp2_approx(Exponent(m, c).of_max(mine.m));
+#pragma unroll
+    for (int d = N / 2; d > 0; d >>= 1) s += __shfl_xor_sync(kAllLanes, s, d);
+    return {m, s};
 }
 
-constexpr int kDistillUnroll = 4;  // vectors a thread has on their way
-
-// Maximum and sum of exp((x - max) c / log2 e) over a part, per thread
-template <class T, int THREADS>
-__device__ __forceinline__ MaxSum scan_part(const T* row, int c0, int c1, float c)
+// Maximum and sum of the row from the warps' (with the other CTAs' of its cluster), in every thread; ends the first of the phases that
+// a barrier parts.
+template <int THREADS>
+__device__ __forceinline__ MaxSum join_row(MaxSum warps, float c, Room<THREADS>& room, int log_parts)
 {
-    constexpr int N = Part<T>::N;
-    const Part<T> part(row, c0, c1);
-    MaxSum mine = {kLowest, 0.0f};
-    const auto take = [&](const float* x, int n) {
-        float top = x[0];
-        for (int i = 1; i < n; ++i) top = fmaxf(top, x[i]);
-        if (top > mine.m) {
-            mine.s *= exp2_approx((mine.m - top) * c);
-            mine.m = top;
-        }
-        for (int i = 0; i < n; ++i) mine.s += exp2_approx((x[i] - mine.m) * c);
-    };
-    const uint4* body = reinterpret_cast<const uint4*>(row + c0 + part.head);
-    int at = threadIdx.x;
-    for (; at + (kDistillUnroll - 1) * THREADS < part.vectors; at += kDistillUnroll * THREADS) {
-        uint4 raw[kDistillUnroll];
-#pragma unroll
-        for (int u = 0; u < kDistillUnroll; ++u) raw[u] = __ldg(body + at + u * THREADS);
-        float x[kDistillUnroll * N];
-#pragma unroll
-        for (int u = 0; u < kDistillUnroll; ++u) {
-            const T* e = reinterpret_cast<const T*>(&raw[u]);
-#pragma unroll
-            for (int i = 0; i < N; ++i) x[u * N + i] = to_f32(e[i]);
-        }
-        float top = x[0];
-#pragma unroll
-        for (int i = 1; i < kDistillUnroll * N; ++i) top = fmaxf(top, x[i]);
-        if (top > mine.m) {
-            mine.s *= exp2_approx((mine.m - top) * c);
-            mine.m = top;
-        }
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < kDistillUnroll * N; ++i) sum[i & 3] += exp2_approx((x[i] - mine.m) * c);
-        mine.s += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    namespace cg = cooperative_groups;
+    constexpr int W = THREADS / 32;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) room.part[threadIdx.x >> 5] = warps;
+    __syncthreads();
+    MaxSum all = join_lanes<W>(room.part[lane % W], c);
+    if (log_parts > 0) {
+        const cg::cluster_group cluster = cg::this_cluster();
+        if (threadIdx.x == 0) room.block = all;
+        cluster.sync();
+        const int parts = 1 << log_parts;
+        all = join_lanes<8>(lane % 8 < parts ? *cluster.map_shared_rank(&room.block, lane % 8) : MaxSum{kLowest, 0.0f}, c);
     }
-    for (; at < part.vectors; at += THREADS) {
-        const uint4 raw = __ldg(body + at);
-        const T* e = reinterpret_cast<const T*>(&raw);
-        float x[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = to_f32(e[i]);
-        take(x, N);
-    }
-    for (int i = threadIdx.x; i < part.head; i += THREADS) {
-        const float x = to_f32(row[c0 + i]);
-        take(&x, 1);
-    }
-    for (int i = part.tail0 + threadIdx.x; i < c1; i += THREADS) {
-        const float x = to_f32(row[i]);
-        take(&x, 1);
-    }
-    return mine;
+    return all;
+}
+// Nobody leaves while another may still read what it left in join_row.
+__device__ __forceinline__ void leave_row(int log_parts)
+{
+    if (log_parts > 0) cooperative_groups::this_cluster().sync();
 }
 
-// dx over a part: first weight t P q everywhere, then the entries' columns again with their p taken off.
+// The largest of the entries' values (NaN where one is), of the warps that have any; read after join_row's barrier.
 template <class T, int THREADS>
-__device__ __forceinline__ void write_part(const DistillParams& p, const T* row, T* out, int c0, int c1, float c, float m, float s, const Teacher& t,
-                                           float mass, float weight)
+__device__ __forceinline__ void leave_top(const Entries<T, THREADS>& entries, Room<THREADS>& room)
 {
-    constexpr int N = Part<T>::N;
-    const float scale = weight * p.temperature * mass / s;
-    const Part<T> part(row, c0, c1);
-    const auto value = [&](T x) { return scale * exp2_approx((to_f32(x) - m) * c); };
-    const uint4* body = reinterpret_cast<const uint4*>(row + c0 + part.head);
-    T* to = out + c0 + part.head;
-    const bool aligned = (reinterpret_cast<uintptr_t>(to) & 15u) == 0;
-    for (int at = threadIdx.x; at < part.vectors; at += kDistillUnroll * THREADS) {
-        uint4 raw[kDistillUnroll];
+    const int warp = threadIdx.x >> 5;
+    float top = -CUDART_INF_F;
+    if (warp * 32 < entries.t.count) {
+        bool broken = false;
+        entries.each([&](int, const Entry& e) {
+            top = fmaxf(top, e.v);
+            broken |= e.v != e.v;
+        });
+        top = warp_max(top);
+        if (__any_sync(kAllLanes, broken)) top = CUDART_NAN_F;
+    }
+    if ((threadIdx.x & 31) == 0) room.top[warp] = top;
+}
+template <int THREADS>
+__device__ __forceinline__ float joined_top(const Room<THREADS>& room)
+{
+    constexpr int W = THREADS / 32;
+    const float top = room.top[(threadIdx.x & 31) % W];
+    return __any_sync(kAllLanes, top != top) ? CUDART_NAN_F : warp_max(top);
+}
+
+// The entries' sums, and the row's loss by the first CTA of the row.  Returns P; t.sum is set after it.
+template <class T, int THREADS>
+__device__ __forceinline__ float finish_loss(const DistillParams& p, const Place& at, const Entries<T, THREADS>& entries, Teacher& t, const Exponent& y,
+                                             float s, Room<THREADS>& room)
+{
+    constexpr int W = THREADS / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // with e = exp((v - top) / t): sum e, and sum e ((v - top) / t - (z - max z))
+    float sum = 0.0f, cross = 0.0f;
+    if (warp * 32 < t.count) {
+        entries.each([&](int, const Entry& e) {
+            const float over = p.log_probs ? e.v : (e.v - t.top) * p.inv_t;
+            const float share = expf(over);
+            sum += share;
+            if (share != 0.0f) cross += share * (over - y.of(e.x) * CUDART_LN2_F);
+        });
+        sum = warp_sum(sum);
+        cross = warp_sum(cross);
+    }
+    if (lane == 0) room.sum[warp] = sum, room.cross[warp] = cross;
+    __syncthreads();
+    sum = room.sum[lane % W];
 #pragma unroll
-        for (int u = 0; u < kDistillUnroll; ++u)
-            if (at + u * THREADS < part.vectors) raw[u] = __ldg(body + at + u * THREADS);
-#pragma unroll
-        for (int u = 0; u < kDistillUnroll; ++u) {
-            const int k = at + u * THREADS;
-            if (k < part.vectors) {
-                const T* e = reinterpret_cast<const T*>(&raw[u]);
-                Pack<T, N> r;
-#pragma unroll
-                for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(value(e[i]));
-                if (aligned) {
-                    *reinterpret_cast<Pack<T, N>*>(to + (long long)k * N) = r;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) to[(long long)k * N + i] = r.v[i];
-                }
-            }
+    for (int d = W / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, d);
+    if (!p.log_probs) t.sum = sum;
+    const float mass = p.log_probs || sum != sum ? sum : 1.0f;
+    if (at.rank == 0 && warp == 0) {
+        cross = warp_sum(lane < W ? room.cross[lane] : 0.0f);
+        if (lane == 0) {
+            const float lse = logf(s), tt = p.temperature * p.temperature;
+            p.loss[at.row] = mass == 0.0f ? 0.0f : tt * (p.log_probs ? cross + mass * lse : cross / sum - logf(sum) + lse);
+            if (p.stats != nullptr) p.stats[at.row] = make_float4(y.m, s, t.top, sum);
         }
     }
-    for (int i = threadIdx.x; i < part.head; i += THREADS) out[c0 + i] = from_f32<T>(value(row[c0 + i]));
-    for (int i = part.tail0 + threadIdx.x; i < c1; i += THREADS) out[i] = from_f32<T>(value(row[i]));
-    // A column that is named more than once is written by its first entry, with all its p in stored order.  Ascending columns
-    // name none twice.
-    bool ascending = true;
-    for (int i = threadIdx.x; i + 1 < t.count; i += THREADS) ascending &= t.column(p, i) < t.column(p, i + 1);
-    const bool distinct = __syncthreads_and(ascending);  // and the rows' writes above come before those below
-    for (int i = threadIdx.x; i < t.count; i += THREADS) {
-        const int col = t.column(p, i);
-        if (col < c0 || col >= c1) continue;
-        float share = t.share(p, i);
-        if (!distinct) {
-            bool first = true;
-            for (int j = 0; j < i && first; ++j) first = t.column(p, j) != col;
-            if (!first) continue;
-            for (int j = i + 1; j < t.count; ++j)
-                if (t.column(p, j) == col) share += t.share(p, j);
-        }
-        out[col] = from_f32<T>(weight * p.temperature * (mass * (exp2_approx((to_f32(row[col]) - m) * c) / s) - share));
-    }
+    return mass;
 }
 
 template <class T, int THREADS>
 __device__ __forceinline__ void zero_part(T* out, int c0, int c1)
 {
-    constexpr int N = Part<T>::N;
     const Part<T> part(out, c0, c1);
-    for (int at = threadIdx.x; at < part.vectors; at += THREADS) *reinterpret_cast<uint4*>(out + c0 + part.head + (long long)at * N) = make_uint4(0, 0, 0, 0);
-    for (int i = threadIdx.x; i < part.head; i += THREADS) out[c0 + i] = from_f32<T>(0.0f);
-    for (int i = part.tail0 + threadIdx.x; i < c1; i += THREADS) out[i] = from_f32<T>(0.0f);
+    for (int at = threadIdx.x; at < part.vectors; at += THREADS) *reinterpret_cast<uint4*>(out + part.first + (long long)at * Part<T>::N) = make_uint4(0, 0, 0, 0);
+    if (part.edge >= 0) out[part.edge] = from_f32<T>(0.0f);
 }
 
-// The loss of a row, and with GRADIENT its dx in the same launch.  Grid: T rows of gridDim.x / T CTAs, a cluster each where that is more than one.
-template <class T, int THREADS, bool GRADIENT, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS) distill_kernel(DistillParams p)
-{
-    namespace cg = cooperative_groups;
-    __shared__ BlockSums<THREADS> room;
-    __shared__ MaxSum of_warp[THREADS / 32];
-    __shared__ MaxSum of_block;
-    wait_for_previous_grid();
-    const int parts = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
-    const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
-    const int row = (int)(blockIdx.x / parts);
-    int c0, c1;
-    part_bounds(p.V, rank, parts, &c0, &c1);
-    const T* x = static_cast<const T*>(p.x) + (long long)row * p.ldx;
-    const float c = p.inv_t * CUDART_L2E_F;
-    Teacher t = teacher_of(p, row);
-
-    if (!p.log_probs) {
-        float top = -CUDART_INF_F;
-        bool broken = false;
-        for (int i = threadIdx.x; i < t.count; i += THREADS) {
-            const float v = __ldg(t.v + i);
-            top = fmaxf(top, v);
-            broken |= v != v;
-        }
-        t.top = block_max<THREADS>(top, room);
-        if (__syncthreads_or(broken)) t.top = CUDART_NAN_F;
-        if (t.top == -CUDART_INF_F) t.count = 0;  // no entry, or none that weighs anything
-    }
-    if (t.count == 0) {  // every CTA of the row leaves here
-        if (rank == 0 && threadIdx.x == 0) {
-            p.loss[row] = 0.0f;
-            if (p.stats != nullptr) p.stats[row] = make_float4(0.0f, 1.0f, -CUDART_INF_F, 1.0f);
-        }
-        if constexpr (GRADIENT) zero_part<T, THREADS>(static_cast<T*>(p.dx) + (long long)row * p.ldd, c0, c1);
-        return;
-    }
-
-    MaxSum mine = scan_part<T, THREADS>(x, c0, c1, c);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        const MaxSum other = {__shfl_xor_sync(kAllLanes, mine.m, d), __shfl_xor_sync(kAllLanes, mine.s, d)};
-        mine = join(mine, other, c);
-    }
-    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = mine;
-    __syncthreads();
-    mine = of_warp[0];
-#pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) mine = join(mine, of_warp[w], c);
-    if constexpr (CLUSTER) {
-        const cg::cluster_group cluster = cg::this_cluster();
-        if (threadIdx.x == 0) of_block = mine;
-        cluster.sync();
-        mine = *cluster.map_shared_rank(&of_block, 0);
-        for (int r = 1; r < parts; ++r) mine = join(mine, *cluster.map_shared_rank(&of_block, r), c);
-        cluster.sync();  // nobody leaves while another reads
-    }
-
-    // with e = exp((v - top) / t): sum e, and sum e ((v - top) / t - (z - max z))
-    float sum = 0.0f, cross = 0.0f;
-    for (int i = threadIdx.x; i < t.count; i += THREADS) {
-        const float v = __ldg(t.v + i);
-        const float over = p.log_probs ? v : (v - t.top) * p.inv_t;
-        const float e = expf(over);
-        sum += e;
-        if (e != 0.0f && rank == 0) cross += e * (over - (to_f32(x[t.column(p, i)]) - mine.m) * p.inv_t);
-    }
-    sum = block_sum<THREADS>(sum, room);
-    if (!p.log_probs) t.sum = sum;
-    const float mass = p.log_probs || sum != sum ? sum : 1.0f;
-    if (rank == 0) {
-        cross = block_sum<THREADS>(cross, room);
-        if (threadIdx.x == 0) {
-            const float lse = logf(mine.s);
-            p.loss[row] = mass == 0.0f ? 0.0f : p.temperature * p.temperature * (p.log_probs ? cross + mass * lse : cross / sum - logf(sum) + lse);
-            if (p.stats != nullptr) p.stats[row] = make_float4(mine.m, mine.s, t.top, sum);
-        }
-    }
-    if constexpr (GRADIENT) {
-        T* out = static_cast<T*>(p.dx) + (long long)row * p.ldd;
-        if (mass == 0.0f) zero_part<T, THREADS>(out, c0, c1);
-        else write_part<T, THREADS>(p, x, out, c0, c1, c, mine.m, mine.s, t, mass, __ldg(p.weight + row * p.weight_stride));
-    }
-}
-
-// dx from the statistics that the loss left.  Grid: T rows of gridDim.x / T CTAs.
+// A row without a teacher: every CTA of it leaves here.
 template <class T, int THREADS>
-__global__ void __launch_bounds__(THREADS) distill_backward_kernel(DistillParams p, int parts)
+__device__ __forceinline__ void leave_out(const DistillParams& p, const Place& at, bool loss, bool gradient)
 {
+    if (loss && at.rank == 0 && threadIdx.x == 0) {
+        p.loss[at.row] = 0.0f;
+        if (p.stats != nullptr) p.stats[at.row] = make_float4(0.0f, 1.0f, -CUDART_INF_F, 1.0f);
+    }
+    if (gradient) zero_part<T, THREADS>(static_cast<T*>(p.dx) + (long long)at.row * p.ldd, at.c0, at.c1);
+}
+
+// A vector of dx at `to`, which need not be aligned
+template <class T>
+__device__ __forceinline__ void store_vector(T* to, const uint4& v, bool aligned)
+{
+    if (aligned) {
+        *reinterpret_cast<uint4*>(to) = v;
+    } else {
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int i = 0; i < Part<T>::N; ++i) to[i] = e[i];
+    }
+}
+
+// The columns of the entries again, over what was written there: their p taken off.  A column that is named more than once is written by its first
+// entry, with all its p in stored order; `repeats`: there may be some.
+template <class T, int THREADS>
+__device__ __forceinline__ void write_entries(const DistillParams& p, const Entries<T, THREADS>& entries, const Teacher& t, const Exponent& y, float scale,
+                                              float weight, T* out, int c0, int c1, bool repeats)
+{
+    entries.each([&](int i, const Entry& e) {
+        if (e.col < c0 || e.col >= c1) return;
+        float share = t.share(p, e.v);
+        if (repeats) {
+            for (int j = 0; j < i; ++j)
+                if (t.column(p, j) == e.col) return;
+            for (int j = i + 1; j < t.count; ++j)
+                if (t.column(p, j) == e.col) share += t.share(p, __ldg(t.v + j));
+        }
+        out[e.col] = from_f32<T>(scale * exp2_approx(y.of(e.x)) - weight * p.temperature * share);
+    });
+}
+
+// dx from the statistics that the loss left.  Grid: T rows of 2^log_parts CTAs.  A part has at most THREADS * NV vectors, all of which are
+// asked for before anything else; two CTAs of 512 threads, or as many smaller ones, share an SM.
+template <class T, int THREADS, int NV>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_gradient_kernel(DistillParams p)
+{
+    constexpr int N = Part<T>::N;
+    constexpr int kNamedWords = THREADS * NV * N / 32 + 2;  // the part's vectors, and what is before and behind them
+    __shared__ unsigned named[kNamedWords];                 // a bit for each column of the part
     wait_for_previous_grid();
-    const int row = (int)(blockIdx.x / parts);
-    int c0, c1;
-    part_bounds(p.V, (int)(blockIdx.x % parts), parts, &c0, &c1);
-    const T* x = static_cast<const T*>(p.x) + (long long)row * p.ldx;
-    T* out = static_cast<T*>(p.dx) + (long long)row * p.ldd;
-    Teacher t = teacher_of(p, row);
-    const float4 stats = __ldg(p.stats + row);
+    const Place at(p);
+    const T* x = static_cast<const T*>(p.x) + (long long)at.row * p.ldx;
+    const Part<T> part(x, at.c0, at.c1);
+    uint4 held[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int k = (int)threadIdx.x + i * THREADS;
+        if (k < part.vectors) held[i] = load_once(x + part.first + k * N);
+    }
+    const float edge = part.edge >= 0 ? to_f32(x[part.edge]) : 0.0f;
+    const float4 stats = __ldg(p.stats + at.row);
+    Teacher t = teacher_of(p, __ldg(p.row_ptr + at.row), __ldg(p.row_ptr + at.row + 1));
     t.top = stats.z;
     t.sum = p.log_probs ? 1.0f : stats.w;
     const float mass = p.log_probs || stats.w != stats.w ? stats.w : 1.0f;
-    if (t.count == 0 || stats.z == -CUDART_INF_F || mass == 0.0f) zero_part<T, THREADS>(out, c0, c1);
-    else write_part<T, THREADS>(p, x, out, c0, c1, p.inv_t * CUDART_L2E_F, stats.x, stats.y, t, mass, __ldg(p.weight + row * p.weight_stride));
+    if (t.count == 0 || stats.z == -CUDART_INF_F || mass == 0.0f) {
+        leave_out<T, THREADS>(p, at, false, true);
+        return;
+    }
+    const Entries<T, THREADS> entries(p, t, x);
+    for (int i = threadIdx.x; i < kNamedWords; i += THREADS) named[i] = 0;
+    const float c = p.inv_t * CUDART_L2E_F;
+    const Exponent y(stats.x, c);
+    const float weight = __ldg(p.weight + at.row * p.weight_stride);
+    const float scale = weight * p.temperature * mass / stats.y;
+    T* out = static_cast<T*>(p.dx) + (long long)at.row * p.ldd;
+    T* to = out + part.first;
+    const bool aligned = (reinterpret_cast<uintptr_t>(to) & 15u) == 0;
+    __syncthreads();
+    const auto write = [&](auto far) {
+        const auto value = [&](Pair v) { return mul2(pair_of(scale, scale), exp2_approx(y.template of<decltype(far)::value>(v))); };
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int k = (int)threadIdx.x + i * THREADS;
+            if (k < part.vectors) store_vector(to + k * N, Words<T>::map(held[i], value), aligned);
+        }
+        if (part.edge >= 0) out[part.edge] = from_f32<T>(scale * exp2_approx(y.of(edge)));
+    };
+    if (y.far) write(std::true_type());
+    else write(std::false_type());
+    bool repeats = false;
+    const bool named_here = (int)(threadIdx.x & ~31u) < t.count;
+    if (named_here) {
+        entries.each([&](int, const Entry& e) {
+            const int k = e.col - at.c0;
+            if (k >= 0 && k < at.c1 - at.c0) repeats |= (atomicOr(&named[k >> 5], 1u << (k & 31)) >> (k & 31)) & 1u;
+        });
+    }
+    repeats = __syncthreads_or(repeats);  // and what was written above comes before what is written below
+    if (named_here) write_entries<T, THREADS>(p, entries, t, y, scale, weight, out, at.c0, at.c1, repeats);
+}
+
+// ---- the ring ------------------------------------------------------------------------------------------
+//
+// WORKERS threads do what is done for every element and one more warp, the manager, all the rest: it starts the copies, makes the teacher's
+// shares, joins maxima and sums (across the cluster too), writes the loss and the entries' columns.  What a row costs beside its elements
+// is then paid by one warp in nine: when all warps took part, that was 600 of 1300 instructions of each, and the kernel was no
+// faster than two plain sweeps (227 us for 1184 rows of 131072 bf16 logits).
+
+constexpr int kListed = 256;  // entries of a row that are kept in shared memory; rows with more read them where they need them
+constexpr int kMostSlots = 3;
+
+struct RingRow {  // what the workers need to write a part of dx
+    float m, scale;
+    int zero, aligned;
+    void* to;
+};
+
+struct RingBlock {  // what a part hands to the others: its maximum and sum, and over its entries sum e (v / t - (z - max z)), sum e
+    float m, s, cross, share;
+};
+
+template <int WORKERS>
+struct RingShared {
+    MaxSum part[kMostSlots][WORKERS / 32];
+    RingRow row[kMostSlots];
+    int vectors[kMostSlots];
+    alignas(16) RingBlock block[2][kDistillMostCtas];
+    float v[3][kListed];  // the entries of this row and the next two; at last what becomes of their columns
+    int col[3][kListed];
+    alignas(8) unsigned long long full[kMostSlots];  // a slot's copies have arrived
+    alignas(8) unsigned long long told[2];           // the blocks of a row have
+    int dead;                                        // something did not within the limit: every row from there on is NaN
+    int joined;                                      // rows whose sums the manager has taken
+};
+
+// Barriers of the CTA by number, for `threads` threads: arriving does not wait.
+__device__ __forceinline__ void barrier_arrive(int number, int threads) { asm volatile("barrier.cta.arrive %0, %1;" ::"r"(number), "r"(threads) : "memory"); }
+__device__ __forceinline__ void barrier_sync(int number, int threads) { asm volatile("barrier.cta.sync %0, %1;" ::"r"(number), "r"(threads) : "memory"); }
+
+// 16 bytes to the same place in the shared memory of CTA `rank` of the cluster, counted by its barrier
+__device__ __forceinline__ void tell(unsigned to, const RingBlock& b, unsigned bar, int rank)
+{
+    asm volatile(
+        "{\n\t.reg .b32 ra, rb;\n\t"
+        "mapa.shared::cluster.u32 ra, %0, %6;\n\t"
+        "mapa.shared::cluster.u32 rb, %1, %6;\n\t"
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [ra], {%2, %3, %4, %5}, [rb];\n\t}" ::"r"(to),
+        "r"(bar), "r"(__float_as_uint(b.m)), "r"(__float_as_uint(b.s)), "r"(__float_as_uint(b.cross)), "r"(__float_as_uint(b.share)), "r"(rank)
+        : "memory");
+}
+
+// Grid: clusters of 2^log_parts CTAs, each with `rows` rows in turn.
+template <class T, int WORKERS, bool GRADIENT>
+__global__ void __launch_bounds__(WORKERS + 32, WORKERS == 32 ? 14 : WORKERS == 128 ? 6 : WORKERS == 256 ? 3 : 1) distill_ring_kernel(DistillParams p)
+{
+    constexpr int N = Part<T>::N, W = WORKERS / 32, UNROLL = 4, ALL = WORKERS + 32;
+    constexpr int kSums = 1, kRow = 1 + kMostSlots, kWritten = 1 + 2 * kMostSlots;  // barriers, one a slot each
+    __shared__ RingShared<WORKERS> sh;
+    extern __shared__ __align__(128) unsigned char ring_smem[];
+    unsigned* named = reinterpret_cast<unsigned*>(ring_smem);  // GRADIENT: a bit for each column of the part
+    unsigned char* ring = ring_smem + p.ring_offset;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int first_row = (int)(blockIdx.x >> p.log_parts) * p.rows;
+    const int rows = min(p.rows, p.T - first_row), parts = 1 << p.log_parts;
+    const float c = p.inv_t * CUDART_L2E_F;
+    volatile int* const dead = &sh.dead;
+
+    if (tid == 0) {
+        for (int k = 0; k < p.slots; ++k) mbar_init(smem_u32(&sh.full[k]), 1);
+        for (int k = 0; k < 2; ++k) mbar_init(smem_u32(&sh.told[k]), 1);
+        sh.dead = 0;
+        sh.joined = 0;
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    if constexpr (GRADIENT) {
+        for (int i = tid; i * 4 < p.ring_offset; i += ALL) named[i] = 0;
+    }
+    wait_for_previous_grid();
+    if (parts > 1) cooperative_groups::this_cluster().sync();  // the others' barriers are there
+    else __syncthreads();
+
+    if (warp < W) {  // ---- workers
+        int slot = 0;
+        unsigned phase = 0;
+        for (int i = 0; i < rows; ++i) {
+            bool arrived = *dead == 0;
+            if (arrived) {
+                arrived = mbar_wait_bounded(smem_u32(&sh.full[slot]), phase);
+                if (!arrived) *dead = 1;
+            }
+            if (!arrived) {  // without copies to wait for, no further ahead of the manager than they would let this warp be
+                volatile int* const joined = &sh.joined;
+                for (unsigned spin = 0; spin < kWaitSpinLimit && *joined + p.slots <= i; ++spin) {}
+            }
+            __syncwarp();
+            const uint4* const from = reinterpret_cast<const uint4*>(ring + slot * p.slot_bytes);
+            const int vectors = arrived ? sh.vectors[slot] : 0;
+            constexpr unsigned none = Words<T>::kMinusInf;
+            unsigned top_words = none;
+            for (int k = tid; k < vectors; k += UNROLL * WORKERS) {
+                uint4 v[UNROLL];
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) v[u] = k + u * WORKERS < vectors ? from[k + u * WORKERS] : make_uint4(none, none, none, none);
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) top_words = max_words<T>(top_words, v[u]);
+            }
+            const Exponent y(warp_max(fmaxf(Words<T>::largest(top_words), kLowest)), c);
+            Pair sum = pair_of(0.0f, 0.0f);
+            const auto add = [&](auto far) {
+                const auto take = [&](const uint4& v) {
+                    Words<T>::each(v, [&](Pair w) { sum = add2(sum, exp2_approx(y.template of<decltype(far)::value>(w))); });
+                };
+                int k = tid;
+                for (; k + (UNROLL - 1) * WORKERS < vectors; k += UNROLL * WORKERS) {
+                    uint4 v[UNROLL];
+#pragma unroll
+                    for (int u = 0; u < UNROLL; ++u) v[u] = from[k + u * WORKERS];
+#pragma unroll
+                    for (int u = 0; u < UNROLL; ++u) take(v[u]);
+                }
+                for (; k < vectors; k += WORKERS) take(from[k]);
+            };
+            if (y.far) add(std::true_type());
+            else add(std::false_type());
+            const float s = warp_sum(arrived ? halves(sum).x + halves(sum).y : CUDART_NAN_F);
+            if (lane == 0) sh.part[slot][warp] = {y.m, s};
+            barrier_arrive(kSums + slot, ALL);
+            if constexpr (GRADIENT) {
+                barrier_sync(kRow + slot, ALL);
+                const RingRow row = sh.row[slot];
+                T* const to = static_cast<T*>(row.to);
+                if (row.zero) {
+                    for (int k = tid; k < vectors; k += WORKERS) store_vector(to + (long long)k * N, make_uint4(0, 0, 0, 0), row.aligned);
+                } else {
+                    const Exponent z(row.m, c);
+                    const auto write = [&](auto far) {
+                        const Pair scale = pair_of(row.scale, row.scale);
+                        const auto value = [&](Pair v) { return mul2(scale, exp2_approx(z.template of<decltype(far)::value>(v))); };
+#pragma unroll 4
+                        for (int k = tid; k < vectors; k += WORKERS) store_vector(to + (long long)k * N, Words<T>::map(from[k], value), row.aligned);
+                    };
+                    if (z.far) write(std::true_type());
+                    else write(std::false_type());
+                }
+                barrier_arrive(kWritten + slot, ALL);
+            }
+            if (++slot == p.slots) slot = 0, phase ^= 1;
+        }
+    } else {  // ---- the manager
+        const int rank = (int)blockIdx.x & (parts - 1);
+        const T* const all_x = static_cast<const T*>(p.x);
+        const auto issue = [&](int i, int slot) {  // the copies of row first_row + i
+            const Place at(p, first_row + i);
+            const T* x = all_x + (long long)at.row * p.ldx;
+            const Part<T> part(x, at.c0, at.c1);
+            if (lane == 0) {
+                const unsigned bar = smem_u32(&sh.full[slot]), to = smem_u32(ring + slot * p.slot_bytes), bytes = (unsigned)part.vectors * 16u;
+                sh.vectors[slot] = part.vectors;
+                mbar_expect_tx(bar, bytes);
+                constexpr unsigned kPiece = 16384;
+                for (unsigned from = 0; from < bytes; from += kPiece)
+                    bulk_copy_g2s(to + from, reinterpret_cast<const char*>(x + part.first) + from, min(kPiece, bytes - from), bar);
+            }
+        };
+        for (int i = 0; i < min(p.slots, rows); ++i) issue(i, i);
+        // Row offsets are asked for four rows ahead, entries two and the part's single elements (a lane each) and the weight one row ahead; a
+        // row's shares are made while the workers write the row before it.
+        const auto offset = [&](int i) { return __ldg(p.row_ptr + first_row + min(i, rows)); };
+        int offsets[5] = {offset(0), offset(1), offset(2), offset(3), 0};  // of row i and the next ones
+        const auto fetch_entries = [&](int i, int from, int to) {
+            const Teacher t = teacher_of(p, from, to);
+            const int buffer = i % 3;
+            if (i < rows && t.count <= kListed) {
+                for (int j = lane; j < t.count; j += 32) {
+                    async_copy_vec<1>(smem_u32(&sh.v[buffer][j]), t.v + j);
+                    async_copy_vec<1>(smem_u32(&sh.col[buffer][j]), t.cols + j);
+                }
+            }
+            async_commit();
+        };
+        const auto edge_column = [&](const Part<T>& part, const Place& at) {
+            const int head = part.first - at.c0, behind = part.first + part.vectors * N + lane - head;
+            return lane < head ? at.c0 + lane : behind < at.c1 ? behind : -1;
+        };
+        const auto fetch_edge = [&](int i) {
+            const Place at(p, first_row + i);
+            const T* x = all_x + (long long)at.row * p.ldx;
+            const int col = edge_column(Part<T>(x, at.c0, at.c1), at);
+            return col >= 0 ? to_f32(x[col]) : -CUDART_INF_F;
+        };
+        const auto value_of = [&](const Teacher& t, int i, int j) { return t.count <= kListed ? sh.v[i % 3][j] : __ldg(t.v + j); };
+        const auto over_of = [&](const Teacher& t, float v) { return p.log_probs ? v : (v - t.top) * p.inv_t; };
+        const auto teach = [&](int i, int from, int to) {  // row i's shares: exp(over_of) / sum; top is -infinity where none weighs anything
+            Teacher t = teacher_of(p, from, to);
+            t.top = -CUDART_INF_F;
+            t.sum = 0.0f;
+            async_wait<1>();  // all but the latest fetch
+            __syncwarp();
+            if (p.log_probs) {
+                if (t.count > 0) t.top = 0.0f;
+            } else {
+                bool broken = false;
+#pragma unroll 4
+                for (int j = lane; j < t.count; j += 32) {
+                    const float v = value_of(t, i, j);
+                    t.top = fmaxf(t.top, v);
+                    broken |= v != v;
+                }
+                t.top = __any_sync(kAllLanes, broken) ? CUDART_NAN_F : warp_max(t.top);
+            }
+            if (t.top != -CUDART_INF_F) {
+#pragma unroll 4
+                for (int j = lane; j < t.count; j += 32) t.sum += expf(over_of(t, value_of(t, i, j)));
+                t.sum = warp_sum(t.sum);
+            }
+            return t;
+        };
+        const auto weight_of = [&](int i) { return GRADIENT ? __ldg(p.weight + (first_row + i) * p.weight_stride) : 0.0f; };
+        fetch_entries(0, offsets[0], offsets[1]);
+        fetch_entries(1, offsets[1], offsets[2]);
+        float next_edge = fetch_edge(0), next_weight = weight_of(0);
+        Teacher next = teach(0, offsets[0], offsets[1]);
+        int slot = 0;
+        unsigned phase = 0;
+        for (int i = 0; i < rows; ++i) {
+            const Place at(p, first_row + i);
+            const T* x = all_x + (long long)at.row * p.ldx;
+            const Part<T> part(x, at.c0, at.c1);
+            const T* const here = reinterpret_cast<const T*>(ring + slot * p.slot_bytes);
+            const auto element = [&](int col) {  // of this part
+                const int k = col - part.first;
+                return to_f32(k >= 0 && k < part.vectors * N ? here[k] : x[col]);
+            };
+            const Teacher t = next;
+            const bool listed = t.count <= kListed, counts = t.top != -CUDART_INF_F;
+            const auto column = [&](int j) { return listed ? min(max(sh.col[i % 3][j], 0), p.V - 1) : t.column(p, j); };
+            const float edge = next_edge, weight = next_weight;
+            offsets[4] = offset(i + 4);
+
+            // While the workers sum.  The entries of the part's columns, relative to the largest of the student's logits there, and the single
+            // elements of the lanes.
+            bool arrived = *dead == 0;
+            if (arrived) {
+                arrived = mbar_wait_bounded(smem_u32(&sh.full[slot]), phase);
+                if (!arrived) *dead = 1;
+            }
+            arrived = __all_sync(kAllLanes, arrived);
+            float cross = 0.0f, share = 0.0f, top = kLowest;
+            if (counts) {
+                for (int j = lane; j < t.count; j += 32) {
+                    const int col = column(j);
+                    if (col >= at.c0 && col < at.c1) top = fmaxf(top, element(col));
+                }
+                top = warp_max(top);
+                const Exponent y(top, c);
+                for (int j = lane; j < t.count; j += 32) {
+                    const int col = column(j);
+                    if (col >= at.c0 && col < at.c1) {
+                        const float over = over_of(t, value_of(t, i, j)), e = expf(over);
+                        share += e;
+                        if (e != 0.0f) cross += e * (over - y.of(element(col)) * CUDART_LN2_F);
+                    }
+                }
+                cross = warp_sum(cross);
+                share = warp_sum(share);
+            }
+            MaxSum edges = {fmaxf(warp_max(edge), kLowest), 0.0f};
+            edges.s = warp_sum(exp2_approx(Exponent(edges.m, c).of(edge)));
+
+            // the part's maximum and sum
+            barrier_sync(kSums + slot, ALL);
+            if (lane == 0) *const_cast<volatile int*>(&sh.joined) = i + 1;
+            constexpr int kJoined = W < 16 ? 16 : 32;
+            const int whose = lane % kJoined;
+            const MaxSum mine = join_lanes<kJoined>(whose < W ? sh.part[slot][whose] : whose == W ? edges : MaxSum{kLowest, 0.0f}, c);
+            if (share != 0.0f) cross -= Exponent(mine.m, c).of_max(top) * CUDART_LN2_F * share;
+            if constexpr (!GRADIENT) {
+                if (arrived && i + p.slots < rows) {  // everybody has read the slot
+                    if (lane == 0) fence_proxy_async_smem();
+                    issue(i + p.slots, slot);
+                }
+            }
+
+            // the row's: every part tells every other
+            RingBlock block = {mine.m, mine.s, cross, share};
+            MaxSum all = mine;
+            if (parts > 1) {
+                const unsigned bar = smem_u32(&sh.told[i & 1]);
+                if (lane == 0) mbar_expect_tx(bar, (unsigned)parts * sizeof(RingBlock));
+                if (lane < parts) tell(smem_u32(&sh.block[i & 1][rank]), block, bar, lane);
+                bool told = *dead == 0 && mbar_wait_bounded(bar, (unsigned)(i >> 1) & 1u);
+                told = __all_sync(kAllLanes, told);
+                if (!told) *dead = 1;
+                block = lane % 8 < parts ? sh.block[i & 1][lane % 8] : RingBlock{kLowest, 0.0f, 0.0f, 0.0f};
+                all = join_lanes<8>({block.m, block.s}, c);
+                if (!told) all.s = CUDART_NAN_F;
+            }
+            const Exponent y(all.m, c);
+            const float mass = !counts ? 0.0f : p.log_probs || t.sum != t.sum ? t.sum : 1.0f;
+            const bool zero = mass == 0.0f;
+            const float scale = weight * p.temperature * mass / all.s;
+            if constexpr (GRADIENT) {
+                T* const to = static_cast<T*>(p.dx) + (long long)at.row * p.ldd + part.first;
+                if (lane == 0) sh.row[slot] = {all.m, scale, zero, (reinterpret_cast<uintptr_t>(to) & 15u) == 0, to};
+                barrier_arrive(kRow + slot, ALL);
+            }
+
+            // while the workers write
+            fetch_entries(i + 2, offsets[2], offsets[3]);
+            if (i + 1 < rows) {
+                next_edge = fetch_edge(i + 1);
+                next_weight = weight_of(i + 1);
+            }
+            if (rank == 0) {
+                float crosses = 0.0f;
+                if (lane < parts) crosses = block.cross - (block.share != 0.0f ? y.of_max(block.m) * CUDART_LN2_F * block.share : 0.0f);
+                crosses = warp_sum(crosses);
+                if (lane == 0) {
+                    const float lse = logf(all.s), tt = p.temperature * p.temperature;
+                    p.loss[at.row] = zero ? 0.0f : tt * (p.log_probs ? crosses + mass * lse : crosses / t.sum - logf(t.sum) + lse);
+                    if (p.stats != nullptr)
+                        p.stats[at.row] = counts ? make_float4(all.m, all.s, t.top, t.sum) : make_float4(0.0f, 1.0f, -CUDART_INF_F, 1.0f);
+                }
+            }
+            if constexpr (GRADIENT) {
+                T* const out = static_cast<T*>(p.dx) + (long long)at.row * p.ldd;
+                const int edge_col = edge_column(part, at);
+                if (edge_col >= 0) out[edge_col] = from_f32<T>(zero ? 0.0f : scale * exp2_approx(y.of(edge)));
+                const auto share_of = [&](int j) {
+                    const float e = expf(over_of(t, value_of(t, i, j)));
+                    return p.log_probs ? e : e / t.sum;
+                };
+                const auto gradient = [&](int col, float taken) {
+                    return scale * exp2_approx(y.of(element(col))) - weight * p.temperature * taken;
+                };
+                const auto inside = [&](int col) { return !zero && col >= at.c0 && col < at.c1; };
+                bool repeats = false;
+                if (!zero) {
+                    for (int j = lane; j < t.count; j += 32) {
+                        const int col = column(j), k = col - at.c0;
+                        if (inside(col)) repeats |= (atomicOr(&named[k >> 5], 1u << (k & 31)) >> (k & 31)) & 1u;
+                    }
+                    repeats = __any_sync(kAllLanes, repeats);
+                    for (int j = lane; j < t.count; j += 32)
+                        if (inside(column(j))) named[(column(j) - at.c0) >> 5] = 0;
+                }
+                const bool ready = listed && !repeats;  // what becomes of the entries' columns is known before the workers are done
+                if (ready) {
+                    for (int j = lane; j < t.count; j += 32)
+                        if (inside(column(j))) sh.v[i % 3][j] = gradient(column(j), share_of(j));
+                }
+                if (i + 1 < rows) next = teach(i + 1, offsets[1], offsets[2]);
+                barrier_sync(kWritten + slot, ALL);  // what the workers wrote comes before what is written here
+                if (!ready) {
+                    for (int j = lane; j < t.count; j += 32) {
+                        const int col = column(j);
+                        if (!inside(col)) continue;
+                        float taken = share_of(j);
+                        if (repeats) {  // a column named more than once is written by its first entry, with all its p in stored order
+                            bool first = true;
+                            for (int q = 0; q < j && first; ++q) first = column(q) != col;
+                            if (!first) continue;
+                            for (int q = j + 1; q < t.count; ++q)
+                                if (column(q) == col) taken += share_of(q);
+                        }
+                        out[col] = from_f32<T>(gradient(col, taken));
+                    }
+                    __syncwarp();
+                }
+                if (arrived && i + p.slots < rows) {  // everybody has read the slot
+                    if (lane == 0) fence_proxy_async_smem();
+                    issue(i + p.slots, slot);
+                }
+                if (ready) {
+                    for (int j = lane; j < t.count; j += 32)
+                        if (inside(column(j))) out[column(j)] = from_f32<T>(sh.v[i % 3][j]);
+                }
+                __syncwarp();  // the row's entries have been read
+            } else if (i + 1 < rows) {
+                next = teach(i + 1, offsets[1], offsets[2]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) offsets[k] = offsets[k + 1];
+            if (++slot == p.slots) slot = 0, phase ^= 1;
+        }
+        async_wait<0>();
+        if (*dead != 0 && lane == 0) {  // no copy may arrive after the CTA has gone: each barrier is at the phase of its last one, or past it
+            for (int k = 0; k < p.slots; ++k) {
+                mbar_wait_bounded(smem_u32(&sh.full[k]), 0);
+                mbar_wait_bounded(smem_u32(&sh.full[k]), 1);
+            }
+        }
+    }
+    if (parts > 1) cooperative_groups::this_cluster().sync();  // nobody leaves while another may still tell it something
+}
+
+// Rows longer than a cluster holds: the same in two sweeps over the part, the second from L2 where it has stayed there.
+constexpr int kLongThreads = 512;
+constexpr int kLongUnroll = 4;
+
+template <class T, bool GRADIENT>
+__global__ void __launch_bounds__(kLongThreads, 2) distill_long_kernel(DistillParams p)
+{
+    constexpr int N = Part<T>::N, THREADS = kLongThreads;
+    __shared__ Room<THREADS> room;
+    wait_for_previous_grid();
+    const Place at(p);
+    const T* x = static_cast<const T*>(p.x) + (long long)at.row * p.ldx;
+    const Part<T> part(x, at.c0, at.c1);
+    Teacher t = teacher_of(p, __ldg(p.row_ptr + at.row), __ldg(p.row_ptr + at.row + 1));
+    if (t.count == 0) {
+        leave_out<T, THREADS>(p, at, true, GRADIENT);
+        return;
+    }
+    const Entries<T, THREADS> entries(p, t, x);
+    const float c = p.inv_t * CUDART_L2E_F;
+    const float edge = part.edge >= 0 ? to_f32(x[part.edge]) : -CUDART_INF_F;
+    const auto load = [&](int k, uint4 (&v)[kLongUnroll]) {
+        constexpr unsigned none = Words<T>::kMinusInf;
+#pragma unroll
+        for (int u = 0; u < kLongUnroll; ++u)
+            v[u] = k + u * THREADS < part.vectors ? __ldg(reinterpret_cast<const uint4*>(x + part.first) + k + u * THREADS) : make_uint4(none, none, none, none);
+    };
+
+    MaxSum mine = {kLowest, 0.0f};
+    for (int k = threadIdx.x; k < part.vectors; k += kLongUnroll * THREADS) {
+        uint4 v[kLongUnroll];
+        load(k, v);
+        unsigned top_words = v[0].x;
+#pragma unroll
+        for (int u = 0; u < kLongUnroll; ++u) top_words = max_words<T>(top_words, v[u]);
+        const Exponent y(fmaxf(mine.m, Words<T>::largest(top_words)), c);
+        if (y.m > mine.m) mine = {y.m, mine.s * exp2_approx(y.of_max(mine.m))};
+        Pair sum = pair_of(0.0f, 0.0f);
+        const auto add = [&](auto far) {
+#pragma unroll
+            for (int u = 0; u < kLongUnroll; ++u)
+                Words<T>::each(v[u], [&](Pair w) { sum = add2(sum, exp2_approx(y.template of<decltype(far)::value>(w))); });
+        };
+        if (y.far) add(std::true_type());
+        else add(std::false_type());
+        mine.s += halves(sum).x + halves(sum).y;
+    }
+    if (part.edge >= 0) {
+        const Exponent y(fmaxf(mine.m, edge), c);
+        mine = {y.m, mine.s * exp2_approx(y.of_max(mine.m)) + exp2_approx(y.of(edge))};
+    }
+    if (!p.log_probs) leave_top<T, THREADS>(entries, room);
+    const MaxSum all = join_row<THREADS>(join_lanes<32>(mine, c), c, room, p.log_parts);
+    if (!p.log_probs) {
+        t.top = joined_top<THREADS>(room);
+        if (t.top == -CUDART_INF_F) {
+            leave_out<T, THREADS>(p, at, true, GRADIENT);
+            leave_row(p.log_parts);
+            return;
+        }
+    }
+    const Exponent y(all.m, c);
+    const float mass = finish_loss<T, THREADS>(p, at, entries, t, y, all.s, room);
+    if constexpr (GRADIENT) {
+        T* out = static_cast<T*>(p.dx) + (long long)at.row * p.ldd;
+        if (mass == 0.0f) {
+            zero_part<T, THREADS>(out, at.c0, at.c1);
+        } else {
+            const float weight = __ldg(p.weight + at.row * p.weight_stride);
+            const float scale = weight * p.temperature * mass / all.s;
+            T* to = out + part.first;
+            const bool aligned = (reinterpret_cast<uintptr_t>(to) & 15u) == 0;
+            const auto value = [&](Pair v) {
+                const float2 w = halves(v);
+                return mul2(pair_of(scale, scale), exp2_approx(pair_of(y.of(w.x), y.of(w.y))));
+            };
+            for (int k = threadIdx.x; k < part.vectors; k += kLongUnroll * THREADS) {
+                uint4 v[kLongUnroll];
+                load(k, v);
+#pragma unroll
+                for (int u = 0; u < kLongUnroll; ++u)
+                    if (k + u * THREADS < part.vectors) store_vector(to + (long long)(k + u * THREADS) * N, Words<T>::map(v[u], value), aligned);
+            }
+            if (part.edge >= 0) out[part.edge] = from_f32<T>(scale * exp2_approx(y.of(edge)));
+            // ascending columns name none twice
+            bool repeats = false;
+            for (int i = threadIdx.x; i + 1 < t.count; i += THREADS) repeats |= t.column(p, i) >= t.column(p, i + 1);
+            repeats = __syncthreads_or(repeats);
+            write_entries<T, THREADS>(p, entries, t, y, scale, weight, out, at.c0, at.c1, repeats);
+        }
+    }
+    leave_row(p.log_parts);
 }
 
 }  // namespace csrspmm_b200

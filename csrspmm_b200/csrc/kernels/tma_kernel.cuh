@@ -18,67 +18,12 @@
 // kStatusWaitTimeout and drains what it had in flight with a second bounded wait.
 #pragma once
 
+#include "async_copy.cuh"
 #include "merge_kernel.cuh"
 
 namespace csrspmm_b200 {
 
 constexpr int kTmaWarps = kMergeThreads / 32;
-
-__device__ __forceinline__ unsigned smem_u32(const void* p)
-{
-    return static_cast<unsigned>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(unsigned bar, unsigned count)
-{
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(unsigned bar, unsigned bytes)
-{
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(unsigned bar, unsigned parity)
-{
-    unsigned ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// false when the limit was reached
-__device__ __forceinline__ bool mbar_wait_bounded(unsigned bar, unsigned parity, unsigned limit = kWaitSpinLimit)
-{
-    for (unsigned spin = 0; spin < limit; ++spin)
-        if (mbar_try_wait(bar, parity)) return true;
-    return false;
-}
-
-// One row of B (bytes % 16 == 0, both addresses 16-byte aligned) into this CTA's shared memory.
-__device__ __forceinline__ void bulk_copy_g2s(unsigned dst, const void* src, unsigned bytes, unsigned bar)
-{
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-        "l"(src), "r"(bytes), "r"(bar)
-        : "memory");
-}
-
-__device__ __forceinline__ void fence_proxy_async_smem()
-{
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
-__device__ __forceinline__ void fence_mbar_init()
-{
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-}
 
 // Static part of the shared memory.  The ring is dynamic: kTmaWarps * ring_stride bytes with
 // ring_stride = max(SLOTS * slot_bytes, 512 * NV), so that a warp's ring can also hold the
