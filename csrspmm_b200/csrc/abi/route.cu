@@ -89,10 +89,14 @@ int csrspmm_b200_route(const csrspmm_b200_route_args* a, int32_t* row_ptr, int32
     p.row_ptr = row_ptr, p.col_idx = col_idx, p.values = values;
     const bool ranks_groups = a->top_groups < a->groups;
     const bool on_x = a->bias == nullptr && (!ranks_groups || a->group_top == 1);
-    const size_t smem = ranks_groups ? (size_t)(kRouteThreads / 32) * 8 * (size_t)a->E : 0;
+    const size_t smem = ranks_groups || !on_x ? (size_t)(kRouteThreads / 32) * 8 * (size_t)a->E : 0;
     CUDA_TRY(for_shape(a, [&](auto zero, auto per) {
+        constexpr int per_lane = decltype(per)::value;
+        const int lanes = p.per_group % per_lane == 0 ? p.per_group / per_lane : 0;
+        for (p.log_group_lanes = 0; 1 << p.log_group_lanes < lanes;) ++p.log_group_lanes;
+        p.group_lanes = lanes > 0 && 1 << p.log_group_lanes == lanes ? lanes : 0;
         auto launch = [&](auto x_c) {
-            constexpr auto kernel = route_kernel<decltype(zero), decltype(per)::value, decltype(x_c)::value>;
+            constexpr auto kernel = route_kernel<decltype(zero), per_lane, decltype(x_c)::value>;
             if (smem > 48 * 1024) {
                 const cudaError_t e = allow_dynamic_smem<kernel>(smem);
                 if (e != cudaSuccess) return e;
