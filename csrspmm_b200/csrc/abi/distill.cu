@@ -83,7 +83,8 @@ cudaError_t launch_gradient(const csrspmm_b200_distill_args* a, DistillParams p,
     });
 }
 
-constexpr int kPartBytes = 65536;         // of a part, as far as clusters go: three CTAs of one slot fit an SM
+constexpr int kPartBytes = 100 * 1024;    // of a part, as far as clusters go: two CTAs of one slot fit an SM (three of up to 64 KB)
+constexpr int kFewBytes = 32768;          // up to here four warps do as well as eight, and six CTAs fit an SM (9000 bf16 columns: 192 -> 143 us for 16384 rows)
 constexpr int kDynamicSmem = 216 * 1024;  // of a CTA, beside RingShared
 
 // The ring kernel's manager walks a row's entries with one warp; where rows have more than this many, all warps of the long kernel do.
@@ -111,6 +112,14 @@ cudaError_t launch_loss(const csrspmm_b200_distill_args* a, DistillParams p, cud
     long long parts = 1;
     while (parts < kDistillMostCtas && ((long long)a->V * size > parts * kPartBytes || too_few(a, parts))) parts *= 2;
     const unsigned grid = cut(a, parts, &p);
+    if (parts == 1 && a->V <= 32 * 8 * (16 / size)) {
+        const unsigned ctas = (unsigned)(((long long)a->T + kShortThreads / 32 - 1) / (kShortThreads / 32));
+        return for_type(a->logit_type, [&](auto zero) {
+            using T = decltype(zero);
+            if (a->V <= 32 * 2 * (16 / size)) return launch_overlapped(distill_short_kernel<T, 2, GRADIENT>, ctas, kShortThreads, 0, st, p);
+            return launch_overlapped(distill_short_kernel<T, 8, GRADIENT>, ctas, kShortThreads, 0, st, p);
+        });
+    }
     const long long slot = (long long)p.per * size, before = GRADIENT ? ((long long)p.per / 32 + 1 + 31) / 32 * 128 : 0;
     if (before + slot > kDynamicSmem || a->nnz / std::max(a->T, 1) > kMostEntries)
         return for_type(a->logit_type, [&](auto zero) {
@@ -120,9 +129,8 @@ cudaError_t launch_loss(const csrspmm_b200_distill_args* a, DistillParams p, cud
     p.ring_offset = (int)before;
     return for_type(a->logit_type, [&](auto zero) {
         using T = decltype(zero);
-        if (p.slot_bytes <= 4096) return launch_ring<T, 32, GRADIENT>(a, p, 14, st);
-        if (p.slot_bytes <= 8192) return launch_ring<T, 128, GRADIENT>(a, p, 6, st);
-        if (p.slot_bytes <= kPartBytes) return launch_ring<T, 256, GRADIENT>(a, p, 3, st);
+        if (p.slot_bytes <= kFewBytes) return launch_ring<T, 128, GRADIENT>(a, p, 6, st);
+        if (p.slot_bytes <= kPartBytes) return launch_ring<T, 256, GRADIENT>(a, p, p.slot_bytes <= 65536 ? 3 : 2, st);
         return launch_ring<T, 512, GRADIENT>(a, p, 1, st);
     });
 }

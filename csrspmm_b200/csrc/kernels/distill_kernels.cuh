@@ -10,8 +10,8 @@
 // run of columns.  Bulk copies bring the run into shared memory and the runs of the next rows behind it, so that memory is never waited for row by
 // row; from there it is read for the maximum, for the sum and for the gradient, and memory gives each row once.  What
 // the parts found meets in distributed shared memory.  The teacher's entries are few: one warp makes their shares.
-// The gradient alone (distill_gradient_kernel) needs no sum: every thread holds up to eight vectors.  Rows that are longer than a
-// cluster's shared memory are read twice (distill_long_kernel).
+// The gradient alone (distill_gradient_kernel) needs no sum: every thread holds up to eight vectors.  Rows that one warp can hold are a
+// warp's (distill_short_kernel); rows that are longer than a cluster's shared memory are read twice (distill_long_kernel).
 //
 // Sums, maxima and the loss are fp32.  Exponentials are 2^y with y = x c - m c, c = log2(e) / t, m a maximum: one fused multiply-add each.  The
 // product m c is rounded once and the same rounded one serves the sum, the loss and the gradient, so that its rounding cancels.  Where m c
@@ -411,6 +411,128 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_gradient_kern
     if (named_here) write_entries<T, THREADS>(p, entries, t, y, scale, weight, out, at.c0, at.c1, repeats);
 }
 
+// Short rows: a warp each, which holds its row in registers, up to NV vectors a lane.  (Under the ring's two warps of a CTA a row of 1500 bf16
+// logits took 15 us from end to end, which 14 CTAs per SM do not hide: 16384 of them 122 us.)
+constexpr int kShortThreads = 256;
+
+template <class T, int NV, bool GRADIENT>
+__global__ void __launch_bounds__(kShortThreads) distill_short_kernel(DistillParams p)
+{
+    constexpr int N = Part<T>::N;
+    wait_for_previous_grid();
+    const int lane = threadIdx.x & 31;
+    const int row = (int)(blockIdx.x * (kShortThreads / 32) + (threadIdx.x >> 5));
+    if (row >= p.T) return;
+    const T* const x = static_cast<const T*>(p.x) + (long long)row * p.ldx;
+    const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+    const int head = min(off ? N - off : 0, p.V), vectors = (p.V - head) / N, behind = head + vectors * N + lane - head;
+    const int edge_col = lane < head ? lane : behind < p.V ? behind : -1;  // fewer than 2 N, a lane each
+    uint4 held[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        constexpr unsigned none = Words<T>::kMinusInf;
+        held[i] = lane + i * 32 < vectors ? load_once(x + head + (lane + i * 32) * N) : make_uint4(none, none, none, none);
+    }
+    const float edge = edge_col >= 0 ? to_f32(x[edge_col]) : -CUDART_INF_F;
+    Teacher t = teacher_of(p, __ldg(p.row_ptr + row), __ldg(p.row_ptr + row + 1));
+    const auto entry = [&](int j) {
+        Entry e;
+        e.col = t.column(p, j);
+        e.v = __ldg(t.v + j);
+        e.x = to_f32(x[e.col]);
+        return e;
+    };
+    Entry first = {};
+    if (lane < t.count) first = entry(lane);
+    const auto each = [&](auto&& f) {
+        if (lane < t.count) f(lane, first);
+        for (int j = lane + 32; j < t.count; j += 32) f(j, entry(j));
+    };
+
+    const float c = p.inv_t * CUDART_L2E_F;
+    unsigned top_words = Words<T>::kMinusInf;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) top_words = max_words<T>(top_words, held[i]);
+    const Exponent y(fmaxf(warp_max(fmaxf(Words<T>::largest(top_words), edge)), kLowest), c);
+    Pair sum = pair_of(0.0f, 0.0f);
+    const auto add = [&](auto far) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i * 32 < vectors) Words<T>::each(held[i], [&](Pair w) { sum = add2(sum, exp2_approx(y.template of<decltype(far)::value>(w))); });
+    };
+    if (y.far) add(std::true_type());
+    else add(std::false_type());
+    const float s = warp_sum(halves(sum).x + halves(sum).y + exp2_approx(y.of(edge)));
+
+    t.top = -CUDART_INF_F;
+    t.sum = 0.0f;
+    if (p.log_probs) {
+        if (t.count > 0) t.top = 0.0f;
+    } else {
+        bool broken = false;
+        each([&](int, const Entry& e) {
+            t.top = fmaxf(t.top, e.v);
+            broken |= e.v != e.v;
+        });
+        t.top = __any_sync(kAllLanes, broken) ? CUDART_NAN_F : warp_max(t.top);
+    }
+    const bool counts = t.top != -CUDART_INF_F;  // some entry weighs something
+    const auto over_of = [&](float v) { return p.log_probs ? v : (v - t.top) * p.inv_t; };
+    float cross = 0.0f;
+    if (counts) {
+        each([&](int, const Entry& e) {
+            const float over = over_of(e.v), share = expf(over);
+            t.sum += share;
+            if (share != 0.0f) cross += share * (over - y.of(e.x) * CUDART_LN2_F);
+        });
+        t.sum = warp_sum(t.sum);
+        cross = warp_sum(cross);
+    }
+    const float mass = !counts ? 0.0f : p.log_probs || t.sum != t.sum ? t.sum : 1.0f;
+    const bool zero = mass == 0.0f;
+    if (lane == 0) {
+        const float lse = logf(s), tt = p.temperature * p.temperature;
+        p.loss[row] = zero ? 0.0f : tt * (p.log_probs ? cross + mass * lse : cross / t.sum - logf(t.sum) + lse);
+        if (p.stats != nullptr) p.stats[row] = counts ? make_float4(y.m, s, t.top, t.sum) : make_float4(0.0f, 1.0f, -CUDART_INF_F, 1.0f);
+    }
+    if constexpr (GRADIENT) {
+        T* const out = static_cast<T*>(p.dx) + (long long)row * p.ldd;
+        T* const to = out + head;
+        const bool aligned = (reinterpret_cast<uintptr_t>(to) & 15u) == 0;
+        const float weight = __ldg(p.weight + row * p.weight_stride), scale = weight * p.temperature * mass / s;
+        const auto write = [&](auto far) {
+            const auto value = [&](Pair v) { return mul2(pair_of(scale, scale), exp2_approx(y.template of<decltype(far)::value>(v))); };
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (lane + i * 32 < vectors) store_vector(to + (lane + i * 32) * N, zero ? make_uint4(0, 0, 0, 0) : Words<T>::map(held[i], value), aligned);
+        };
+        if (y.far) write(std::true_type());
+        else write(std::false_type());
+        if (edge_col >= 0) out[edge_col] = from_f32<T>(zero ? 0.0f : scale * exp2_approx(y.of(edge)));
+        if (zero) return;
+        bool repeats = false;  // ascending columns name none twice, nor do 32 that all differ
+        if (t.count <= 32) {
+            const unsigned same = __match_any_sync(kAllLanes, lane < t.count ? first.col : -1 - lane);
+            repeats = __any_sync(kAllLanes, (same & (same - 1)) != 0);
+        } else {
+            for (int j = lane; j + 1 < t.count; j += 32) repeats |= t.column(p, j) >= t.column(p, j + 1);
+            repeats = __any_sync(kAllLanes, repeats);
+        }
+        __syncwarp();  // what was written above comes before what is written below
+        const auto share_of = [&](float v) { return p.log_probs ? expf(v) : expf(over_of(v)) / t.sum; };
+        each([&](int j, const Entry& e) {
+            float taken = share_of(e.v);
+            if (repeats) {  // a column named more than once is written by its first entry, with all its p in stored order
+                for (int q = 0; q < j; ++q)
+                    if (t.column(p, q) == e.col) return;
+                for (int q = j + 1; q < t.count; ++q)
+                    if (t.column(p, q) == e.col) taken += share_of(__ldg(t.v + q));
+            }
+            out[e.col] = from_f32<T>(scale * exp2_approx(y.of(e.x)) - weight * p.temperature * taken);
+        });
+    }
+}
+
 // ---- the ring ------------------------------------------------------------------------------------------
 //
 // WORKERS threads do what is done for every element and one more warp, the manager, all the rest: it starts the copies, makes the teacher's
@@ -463,7 +585,7 @@ __device__ __forceinline__ void tell(unsigned to, const RingBlock& b, unsigned b
 
 // Grid: clusters of 2^log_parts CTAs, each with `rows` rows in turn.
 template <class T, int WORKERS, bool GRADIENT>
-__global__ void __launch_bounds__(WORKERS + 32, WORKERS == 32 ? 14 : WORKERS == 128 ? 6 : WORKERS == 256 ? 3 : 1) distill_ring_kernel(DistillParams p)
+__global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 256 ? 3 : 1) distill_ring_kernel(DistillParams p)
 {
     constexpr int N = Part<T>::N, W = WORKERS / 32, UNROLL = 4, ALL = WORKERS + 32;
     constexpr int kSums = 1, kRow = 1 + kMostSlots, kWritten = 1 + 2 * kMostSlots;  // barriers, one a slot each

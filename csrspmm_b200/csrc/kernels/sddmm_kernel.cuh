@@ -14,7 +14,7 @@
 namespace csrspmm_b200 {
 
 constexpr int kSddmmThreads = 256;
-constexpr int kSddmmMostEntries = 512;  // of a CTA's run
+constexpr int kSddmmMostEntries = 1024;  // of a CTA's run
 
 struct SddmmParams {
     int M, Kd, nvec;  // columns in vectors of VW
@@ -87,10 +87,12 @@ __global__ void __launch_bounds__(kSddmmThreads) sddmm_kernel(SddmmParams p)
         if (at >= 0 && at < n) atomicMax(&row_of[at], r - r0);
     }
     __syncthreads();
-    {  // running maximum over the run, two entries a thread
-        static_assert(kSddmmMostEntries == 2 * kSddmmThreads, "two entries a thread");
-        const int a = row_of[2 * tid], b = max(a, row_of[2 * tid + 1]);
-        int upto = b;
+    {  // running maximum over the run, kEach entries a thread
+        constexpr int kEach = kSddmmMostEntries / kSddmmThreads;
+        int mine[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) mine[i] = i > 0 ? max(mine[i - 1], row_of[kEach * tid + i]) : row_of[kEach * tid];
+        int upto = mine[kEach - 1];
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int v = __shfl_up_sync(kAllLanes, upto, d);
@@ -101,8 +103,8 @@ __global__ void __launch_bounds__(kSddmmThreads) sddmm_kernel(SddmmParams p)
         if (lane == 0) before = 0;
         __syncthreads();
         for (int w = 0; w < warp; ++w) before = max(before, warp_last[w]);
-        row_of[2 * tid] = r0 + max(before, a);
-        row_of[2 * tid + 1] = r0 + max(before, b);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) row_of[kEach * tid + i] = r0 + max(before, mine[i]);
     }
     __syncthreads();
 
