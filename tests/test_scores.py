@@ -157,7 +157,7 @@ def test_nothing_is_compiled_that_no_call_launches(fake):
                 assert fake.csrspmm_b200_route(C.byref(a), P, P, P, None) == 0
                 assert fake.csrspmm_b200_route_backward(C.byref(a), P, P, P, 1, P, E, None) == 0
         for T in (1, 8, 4000):
-            for V in (1, 1000, 6000, 8192, 8193, 15000, 30000, 70000, 300000, 3_000_000):
+            for V in (1, 1000, 6000, 8192, 8193, 15000, 30000, 70000, 300000, 600_000, 3_000_000):
                 d = _distill(T=T, V=V, ld=V, logit_type=kind)
                 assert fake.csrspmm_b200_distill(C.byref(d), P, P, None) == 0
                 assert fake.csrspmm_b200_distill_grad(C.byref(d), P, 1, P, P, V, None) == 0
