@@ -18,8 +18,9 @@ template <int L, int NV, int VW, bool LOOP>
 cudaError_t launch(SddmmParams p, cudaStream_t st)
 {
     constexpr int groups = kSddmmThreads / L;
-    // as many entries for each group of lanes as still give every SM several CTAs, and no more than the row table holds
-    const long long per_group = std::clamp<long long>(p.nnz / ((long long)kSms * 8 * groups), 1, kSddmmMostEntries / groups);
+    // whole waves of the four CTAs that an SM runs, each with the same number of entries, as many as the row table holds at most
+    const long long wave = 4LL * kSms, waves = (p.nnz + wave * kSddmmMostEntries - 1) / (wave * kSddmmMostEntries);
+    const long long per_group = std::clamp<long long>((p.nnz + waves * wave * groups - 1) / (waves * wave * groups), 1, kSddmmMostEntries / groups);
     p.run = (int)per_group * groups;
     const unsigned grid = (unsigned)(((long long)p.nnz + p.run - 1) / p.run);
     return launch_overlapped(sddmm_kernel<L, NV, VW, LOOP>, grid, kSddmmThreads, 0, st, p);

@@ -62,6 +62,18 @@ __device__ __forceinline__ float dot(const Vec<VW>& a, const Vec<VW>& b, float s
     }
 }
 
+// A vector of a row of B that is too wide to be met again in L1: kept out of it, where G's row serves several entries (a training step of
+// 4096 rows of 8 entries, 2048 columns: 213 -> 205 us).  Narrow rows are left in: on a graph that is worth more than the room (262 144 rows of 16, 128 columns: 220 against 306 us).
+__device__ __forceinline__ void load_past_l1(Vec<4>& r, const float* p)
+{
+    asm("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(r.v.x), "=f"(r.v.y), "=f"(r.v.z), "=f"(r.v.w) : "l"(p));
+}
+__device__ __forceinline__ void load_past_l1(Vec<2>& r, const float* p)
+{
+    asm("ld.global.nc.L1::no_allocate.v2.f32 {%0, %1}, [%2];" : "=f"(r.v.x), "=f"(r.v.y) : "l"(p));
+}
+__device__ __forceinline__ void load_past_l1(Vec<1>& r, const float* p) { asm("ld.global.nc.L1::no_allocate.f32 %0, [%1];" : "=f"(r.v) : "l"(p)); }
+
 // LOOP: rows wider than L * NV vectors, in steps of that many
 template <int L, int NV, int VW, bool LOOP>
 __global__ void __launch_bounds__(kSddmmThreads) sddmm_kernel(SddmmParams p)
@@ -165,7 +177,7 @@ __global__ void __launch_bounds__(kSddmmThreads) sddmm_kernel(SddmmParams p)
 #pragma unroll
                     for (int v = 0; v < NV; ++v) {
                         if (c + v * L < p.nvec) {
-                            b[v].load_nc(fb + (c + v * L) * VW);
+                            load_past_l1(b[v], fb + (c + v * L) * VW);
                             g[v].load_nc(fg + (c + v * L) * VW);
                         } else {
                             b[v].zero();
