@@ -542,6 +542,9 @@ __global__ void __launch_bounds__(kShortThreads) distill_short_kernel(DistillPar
 
 constexpr int kListed = 256;  // entries of a row that are kept in shared memory; rows with more read them where they need them
 constexpr int kMostSlots = 3;
+// Attempts of a wait for the other parts of a row, which may still be at the row before: one of many entries that name columns twice
+// takes its manager the square of their number.
+constexpr unsigned kToldLimit = 64 * kWaitSpinLimit;
 
 struct RingRow {  // what the workers need to write a part of dx
     float m, scale;
@@ -823,7 +826,7 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
                 const unsigned bar = smem_u32(&sh.told[i & 1]);
                 if (lane == 0) mbar_expect_tx(bar, (unsigned)parts * sizeof(RingBlock));
                 if (lane < parts) tell(smem_u32(&sh.block[i & 1][rank]), block, bar, lane);
-                bool told = *dead == 0 && mbar_wait_bounded(bar, (unsigned)(i >> 1) & 1u);
+                bool told = *dead == 0 && mbar_wait_bounded(bar, (unsigned)(i >> 1) & 1u, kToldLimit);
                 told = __all_sync(kAllLanes, told);
                 if (!told) *dead = 1;
                 block = lane % 8 < parts ? sh.block[i & 1][lane % 8] : RingBlock{kLowest, 0.0f, 0.0f, 0.0f};

@@ -8,6 +8,10 @@ through ``csrspmm_b200_spmm`` on torch's *current* stream of the tensors' device
 call raises instead of returning an unwritten C.  ``spmm``, the five ops and ``SpmmCall`` reach the library
 through the CPython binding (csrc/torch/binding.cpp), which also makes the argument checks; everything that is
 called once per matrix goes through ctypes.
+
+Next to the products stand the operators that make, learn and compare sparse rows of scores: ``route`` (dense scores to a CSR matrix by
+rank), ``sddmm`` and ``weighted_spmm`` (the gradient for stored values), ``distill_loss`` (a CSR matrix of a teacher's logits against a
+student's dense ones).
 """
 from __future__ import annotations
 

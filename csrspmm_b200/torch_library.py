@@ -12,7 +12,9 @@ The reference's Python ops are plain pybind functions (torch_csrspmm/binding.cpp
 * ``CsrMatrix``: keeps the three arrays, the longest row (so AUTO can pick the row kernel), the cached
   transpose and, per dense width, the matrix's schedule (``csrspmm_b200_schedule_create``) together.
 
-Gradients with respect to the stored values of A (a sampled dense-dense product) are not provided.
+``spmm`` and ``CsrMatrix`` have no gradient for the stored values of A; ``torch.ops.csrspmm_b200.weighted_spmm`` does (``sddmm``, a dense
+product sampled at A's pattern), for matrices whose entries are learnt.  ``route`` makes such a matrix from dense scores, ``distill_loss``
+compares one with dense logits; both are described where users find them, in ``csrspmm_b200.ops``.
 """
 from __future__ import annotations
 

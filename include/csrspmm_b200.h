@@ -357,7 +357,8 @@ int csrspmm_b200_transpose(int32_t M, int32_t Kd, int64_t nnz, const int32_t* ro
  *     k largest c of the top_groups best groups are taken (ties: the lower index), as exact arithmetic would
  *     value = scale * s / (sum of the s taken)  with renormalize, else scale * s
  * Rows hold exactly k entries with ascending columns.  An x of -infinity is an expert that is not available: it is
- * ranked behind all others of the groups taken and its value is 0; where nothing is available all k values are 0.  A row with a
+ * ranked behind all others of the groups taken and its value is 0; where nothing is available all k values are 0.  A bias of -infinity or
+ * NaN ranks an expert there too.  A row with a
  * NaN (softmax: or +infinity) has distinct columns inside the matrix and values of NaN.
  * Scores are device memory, fp32, fp16 or bf16, `ld` elements from row to row; everything is computed in fp32, and in 64 bits where
  * two choices are nearer than that tells apart.  E at most 1024, k and groups at most 32. */
@@ -399,7 +400,7 @@ int csrspmm_b200_sddmm(int32_t M, int32_t Kd, int32_t Nd, int64_t nnz, const int
  *     loss = t^2 * sum_i p_i (ln p_i - z[col_i] + logsumexp z)
  *     dlogits_j = weight * t * (P q_j - sum of the p_i with col_i = j)
  * A row without entries, or with none that weighs anything, has loss 0 and gradient 0 whatever its logits hold.  Entries may come in any
- * order; a column named twice counts with both.  A column outside [0, V) counts as the nearest one inside.
+ * order; a column named twice counts with both (a row's gradient then takes time that grows with the square of its entries).  A column outside [0, V) counts as the nearest one inside.
  * Logits are fp32, fp16 or bf16, computed with in fp32. */
 typedef struct csrspmm_b200_distill_args {
     uint32_t struct_size; /* sizeof(csrspmm_b200_distill_args), checked */

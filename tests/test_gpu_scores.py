@@ -415,7 +415,7 @@ def teacher(T, V, lens, seed, spread=3.0):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("T,V,k", [(1, 1, 1), (3, 7, 7), (5, 100, 8), (40, 1000, 3), (2, 4097, 64), (300, 513, 10), (9, 8192, 16), (7, 8195, 16), (2, 40001, 100),
-                                   (1, 131072, 64), (1, 262145, 5), (3, 65536, 1000), (5000, 700, 4), (9000, 3000, 6),
+                                   (1, 131072, 64), (1, 262145, 5), (3, 65536, 1000), (5000, 700, 4), (9000, 3000, 6), (2, 1_000_003, 9),
                                    (1500, 20000, 12)])
 def test_distill(cuda_lib, dtype, T, V, k):
     x = (4 * torch.randn(T, V, device="cuda", generator=_gen(V + T))).to(dtype)
@@ -438,7 +438,7 @@ def test_distill_of_ragged_rows(cuda_lib, dtype, t, log_probs):
 
 
 @pytest.mark.parametrize("log_probs", [False, True])
-@pytest.mark.parametrize("V", [300, 20000])
+@pytest.mark.parametrize("V", [300, 20000, 150_000, 470_000])
 def test_distill_of_masked_places(cuda_lib, log_probs, V):
     T = 9
     rp, ci, va = teacher(T, V, [6] * T, 8)
@@ -501,6 +501,13 @@ def test_distill_counts_a_column_named_twice_with_both(cuda_lib):
     check_distill(x, rp, ci, va)
     a, b = ops.distill_loss_grad(x, rp, ci, va), ops.distill_loss_grad(x, rp, ci, va)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("V,k", [(1500, 300), (9001, 600), (60000, 300)])
+def test_distill_of_many_entries_with_repeated_columns(cuda_lib, V, k):
+    rp, ci, va = teacher(5, V, [k, 10, k, 0, 7], 21)
+    ci[::3] = ci[1::3][: len(ci[::3])] if len(ci[1::3]) >= len(ci[::3]) else torch.cat([ci[1::3], ci[:1]])[: len(ci[::3])]
+    check_distill(torch.randn(5, V, device="cuda", generator=_gen(22)), rp, ci, va)
 
 
 @pytest.mark.parametrize("k", [3000, 9001])
@@ -668,6 +675,95 @@ def test_on_another_stream_and_replayed_from_a_graph(cuda_lib):
         torch.cuda.synchronize()
         want = step(*[v.detach().clone().requires_grad_(True) for v in eager])
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_padding_behind_rows_is_left_alone(cuda_lib):
+    """The C ABI writes rows of the given width and nothing behind them, at any alignment."""
+    import ctypes as C
+    from csrspmm_b200 import _lib
+    L = _lib.lib()
+    for dtype, kind in ((torch.float32, 0), (torch.bfloat16, 2)):
+        for T, V, k in ((3, 37, 4), (5, 1001, 8), (4, 9003, 8), (2, 70001, 8), (3, 5, 2)):
+            x = torch.randn(T, V, device="cuda", generator=_gen(V)).to(dtype)
+            rp, ci, va = teacher(T, V, [k] * T, 40)
+            loss, stats, w = torch.empty(T, device="cuda"), torch.empty(4 * T, device="cuda"), torch.ones(T, device="cuda")
+            a = _lib.DistillArgs(C.sizeof(_lib.DistillArgs), T, V, kind, x.data_ptr(), V, ci.numel(), rp.data_ptr(), ci.data_ptr(), va.data_ptr(), 1.0, 0)
+            want = ops.distill_loss_grad(x, rp, ci, va)[1]
+            for pad in (1, 3, 8):
+                out = torch.full((T + 1, V + pad), 7.0, device="cuda", dtype=dtype)
+                assert L.csrspmm_b200_distill_grad(C.byref(a), w.data_ptr(), 1, loss.data_ptr(), out[0, 1:].data_ptr(), V + pad, None) == 0
+                flat = out.flatten()[1 : 1 + T * (V + pad)].view(T, V + pad)
+                assert torch.equal(flat[:, :V], want) and (flat[:, V:] == 7).all() and out[0, 0] == 7
+                out.fill_(7.0)
+                assert L.csrspmm_b200_distill(C.byref(a), loss.data_ptr(), stats.data_ptr(), None) == 0
+                assert L.csrspmm_b200_distill_backward(C.byref(a), stats.data_ptr(), w.data_ptr(), 1, out.data_ptr(), V + pad, None) == 0
+                assert torch.allclose(out[:T, :V].float(), want.float(), rtol=2.0 ** -7, atol=1e-6) and (out[:T, V:] == 7).all() and (out[T] == 7).all()
+        x = torch.randn(9, 60, device="cuda", generator=_gen(1)).to(dtype)
+        rp, ci, va = ops.route(x, 5)
+        r = _lib.RouteArgs(struct_size=C.sizeof(_lib.RouteArgs), T=9, E=60, k=5, scores=x.data_ptr(), ld=60, score_type=kind, score=0, groups=1, top_groups=1,
+                           group_top=1, renormalize=1, scale=1.0)
+        out = torch.full((10, 63), 7.0, device="cuda", dtype=dtype)
+        g = torch.randn(45, device="cuda", generator=_gen(2))
+        assert L.csrspmm_b200_route_backward(C.byref(r), ci.data_ptr(), va.data_ptr(), g.data_ptr(), 1, out.data_ptr(), 63, None) == 0
+        want = torch.ops.csrspmm_b200.route_backward(g, x, ci, va, 5, "softmax", True, 1.0)
+        assert torch.equal(out[:9, :60], want) and (out[:9, 60:] == 7).all() and (out[9] == 7).all()
+        guard = torch.full((60,), 7, dtype=torch.int32, device="cuda")
+        values = torch.full((60,), 7.0, device="cuda")
+        offsets = torch.full((20,), 7, dtype=torch.int32, device="cuda")
+        assert L.csrspmm_b200_route(C.byref(r), offsets.data_ptr(), guard.data_ptr(), values.data_ptr(), None) == 0
+        assert torch.equal(offsets[:10], rp) and (offsets[10:] == 7).all()
+        assert torch.equal(guard[:45], ci) and (guard[45:] == 7).all() and torch.equal(values[:45], va) and (values[45:] == 7).all()
+    out = torch.full((40,), 7.0, device="cuda")
+    rp, ci, _ = _csr(10, 8, [3] * 10, 11)
+    G, B = torch.randn(10, 24, device="cuda", generator=_gen(6)), torch.randn(8, 24, device="cuda", generator=_gen(7))
+    assert L.csrspmm_b200_sddmm(10, 8, 24, 30, rp.data_ptr(), ci.data_ptr(), G.data_ptr(), 24, B.data_ptr(), 24, 1.0, out.data_ptr(), None) == 0
+    assert torch.equal(out[:30], ops.sddmm(rp, ci, G, B)) and (out[30:] == 7).all()
+
+
+def test_two_threads_at_once(cuda_lib):
+    import threading
+    x = torch.randn(500, 64, device="cuda", generator=_gen(50))
+    logits = torch.randn(40, 20001, device="cuda", generator=_gen(51))
+    rp, ci, va = teacher(40, 20001, [9] * 40, 52)
+    want = [*ops.route(x, 6, score="sigmoid", bias=x[0].contiguous()), *ops.distill_loss_grad(logits, rp, ci, va)]
+    torch.cuda.synchronize()
+    found = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                leaf = logits.detach().requires_grad_(True)
+                got = [*ops.route(x, 6, score="sigmoid", bias=x[0].contiguous()), *ops.distill_loss_grad(logits, rp, ci, va)]
+                ops.distill_loss(leaf, rp, ci, va).sum().backward()
+                torch.cuda.current_stream().synchronize()
+                found.append(all(torch.equal(a, b) for a, b in zip(got, want)) and torch.allclose(leaf.grad, want[4], rtol=1e-5, atol=1e-8))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert len(found) == 80 and all(found)
+
+
+def test_what_was_saved_and_then_changed_is_refused(cuda_lib):
+    x = torch.randn(6, 32, device="cuda", generator=_gen(60))
+    leaf = x.clone().requires_grad_(True)
+    h = leaf * 1.0
+    va = ops.route(h, 4, renormalize=False)[2]
+    with torch.no_grad():
+        h.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        va.sum().backward()
+    rp, ci, t = teacher(6, 32, [3] * 6, 61)
+    h = leaf * 1.0
+    loss = ops.distill_loss(h, rp, ci, t)
+    with torch.no_grad():
+        t.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+    with torch.inference_mode():
+        assert not ops.route(leaf, 4)[2].requires_grad and not ops.distill_loss(leaf, rp, ci, t).requires_grad
+    with torch.no_grad():
+        assert not ops.route(leaf, 4)[2].requires_grad and not ops.weighted_spmm(rp, ci, t.requires_grad_(True), torch.randn(32, 5, device="cuda")).requires_grad
 
 
 def test_registration(cuda_lib):
