@@ -97,7 +97,7 @@ int csrspmm_b200_route(const csrspmm_b200_route_args* a, int32_t* row_ptr, int32
         p.group_lanes = lanes > 0 && 1 << p.log_group_lanes == lanes ? lanes : 0;
         auto launch = [&](auto x_c) {
             constexpr auto kernel = route_kernel<decltype(zero), per_lane, decltype(x_c)::value>;
-            if (smem > 48 * 1024) {
+            if (smem > 40 * 1024) {  // 48 KB without asking, the kernel's own 1 KB among them
                 const cudaError_t e = allow_dynamic_smem<kernel>(smem);
                 if (e != cudaSuccess) return e;
             }

@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kShortThreads) distill_short_kernel(DistillPar
 // faster than two plain sweeps (227 us for 1184 rows of 131072 bf16 logits).
 
 constexpr int kListed = 256;  // entries of a row that are kept in shared memory; rows with more read them where they need them
-constexpr int kMostSlots = 3;
+constexpr int kMostSlots = 2;
 // Attempts of a wait for the other parts of a row, which may still be at the row before: one of many entries that name columns twice
 // takes its manager the square of their number.
 constexpr unsigned kToldLimit = 64 * kWaitSpinLimit;

@@ -107,7 +107,7 @@ def test_route(cuda_lib, dtype, T, E, k, score, renormalize):
     check_route(x, k, score=score, renormalize=renormalize, bias=bias)
 
 
-@pytest.mark.parametrize("E,groups,top_groups,group_top,k", [(64, 8, 4, 2, 8), (60, 4, 1, 2, 6), (60, 5, 2, 1, 3), (256, 8, 4, 2, 8), (256, 32, 3, 2, 8),
+@pytest.mark.parametrize("E,groups,top_groups,group_top,k", [(64, 8, 4, 2, 8), (640, 10, 4, 1, 5), (752, 8, 2, 2, 8), (768, 8, 2, 2, 8), (769, 1, 1, 1, 8), (60, 4, 1, 2, 6), (60, 5, 2, 1, 3), (256, 8, 4, 2, 8), (256, 32, 3, 2, 8),
                                                              (96, 3, 2, 1, 16), (512, 16, 5, 2, 4), (1024, 4, 3, 2, 8), (32, 32, 7, 1, 7)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("with_bias", [False, True])
