@@ -720,6 +720,47 @@ def test_padding_behind_rows_is_left_alone(cuda_lib):
     assert torch.equal(out[:30], ops.sddmm(rp, ci, G, B)) and (out[30:] == 7).all()
 
 
+def test_more_elements_than_32_bits_count(cuda_lib):
+    """Rows that begin beyond 2^31 elements, in each operator."""
+    T, V = 16_500, 131_100
+    x = torch.zeros(T, V, device="cuda", dtype=torch.bfloat16)
+    last = torch.arange(T - 3, T, device="cuda")
+    x[-3:] = torch.randn(3, V, device="cuda", generator=_gen(70)).bfloat16()
+    lens = torch.zeros(T, dtype=torch.long)
+    lens[-3:] = 20
+    rp, ci, va = teacher(T, V, lens, 71)
+    g = torch.ones(T, device="cuda")
+    loss, dx = ops.distill_loss_grad(x, rp, ci, va, g)
+    leaf = x.requires_grad_(True)
+    again = ops.distill_loss(leaf, rp, ci, va)
+    (dx2,) = torch.autograd.grad(again, leaf, g)
+    small = teacher(3, V, [20] * 3, 71)  # the same entries
+    want = ops.distill_loss_grad(x.detach()[last], *small)
+    assert torch.equal(small[1], ci) and torch.equal(small[2], va)
+    assert torch.equal(loss[-3:], want[0]) and torch.equal(again.detach()[-3:], want[0]) and (loss[:-3] == 0).all()
+    assert torch.equal(dx[-3:], want[1]) and torch.allclose(dx2[-3:].float(), want[1].float(), rtol=2.0 ** -7, atol=1e-7)
+    assert not dx[:100].any() and not dx2[T - 100 : T - 3].any()
+    del x, leaf, dx, dx2, again
+    T, E = 8_400_000, 256
+    x = torch.zeros(T, E, device="cuda", dtype=torch.bfloat16)
+    x[-2:] = torch.randn(2, E, device="cuda", generator=_gen(72)).bfloat16()
+    x.requires_grad_(True)
+    rp, ci, va = ops.route(x, 4, score="sigmoid", renormalize=False)
+    (dx,) = torch.autograd.grad(va.sum(), x)
+    few = x.detach()[-2:].clone().requires_grad_(True)
+    want = ops.route(few, 4, score="sigmoid", renormalize=False)
+    (want_dx,) = torch.autograd.grad(want[2].sum(), few)
+    assert torch.equal(ci[-8:], want[1]) and torch.equal(va[-8:], want[2]) and torch.equal(dx[-2:], want_dx) and int(rp[-1]) == 4 * T
+    assert torch.equal(ci[:4], torch.arange(4, device="cuda", dtype=torch.int32))
+    del x, dx, va
+    Kd, Nd = (1 << 22) + 7, 513
+    B = torch.empty(Kd, Nd, device="cuda").normal_(generator=_gen(73))
+    G = torch.randn(5, Nd, device="cuda", generator=_gen(74))
+    rp = torch.tensor([0, 2, 2, 5, 6, 8], dtype=torch.int32, device="cuda")
+    ci = torch.tensor([Kd - 1, 0, Kd - 2, Kd - 3, 5, Kd - 1, 4_190_000, Kd - 1], dtype=torch.int32, device="cuda")
+    check_sddmm(rp, ci, G, B)
+
+
 def test_two_threads_at_once(cuda_lib):
     import threading
     x = torch.randn(500, 64, device="cuda", generator=_gen(50))
