@@ -48,7 +48,8 @@ EXPORTED_SYMBOLS = (
     "csrspmm_b200_e2m1_quantize_device", "csrspmm_b200_transpose", "csrspmm_b200_transpose_workspace_bytes",
     "csrspmm_b200_spmm_tiled", "csrspmm_b200_tiled_workspace_bytes", "csrspmm_b200_tiled_panel_rows",
     "csrspmm_b200_schedule_create", "csrspmm_b200_schedule_destroy", "csrspmm_b200_schedule_info_get",
-    "csrspmm_b200_route", "csrspmm_b200_route_backward", "csrspmm_b200_sddmm", "csrspmm_b200_distill",
+    "csrspmm_b200_route", "csrspmm_b200_route_backward", "csrspmm_b200_sddmm", "csrspmm_b200_spmm_transposed",
+    "csrspmm_b200_spmm_transposed_pays", "csrspmm_b200_distill",
     "csrspmm_b200_distill_backward", "csrspmm_b200_distill_grad",
 )
 
@@ -221,10 +222,13 @@ def lib() -> C.CDLL:
                                               C.c_void_p]
     L.csrspmm_b200_sddmm.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
                                      C.c_int64, C.c_float, C.c_void_p, C.c_void_p]
+    L.csrspmm_b200_spmm_transposed_pays.argtypes = [C.c_int32, C.c_int32, C.c_int64]
+    L.csrspmm_b200_spmm_transposed.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
+                                               C.c_float, C.c_void_p, C.c_int64, C.c_void_p]
     L.csrspmm_b200_distill.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p, C.c_void_p]
     L.csrspmm_b200_distill_backward.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]
     L.csrspmm_b200_distill_grad.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
-    for name in ("route", "route_backward", "sddmm", "distill", "distill_backward", "distill_grad"):
+    for name in ("route", "route_backward", "sddmm", "spmm_transposed", "spmm_transposed_pays", "distill", "distill_backward", "distill_grad"):
         getattr(L, "csrspmm_b200_" + name).restype = C.c_int
     if L.csrspmm_b200_abi_version() != ABI_VERSION:
         raise LibraryMissing(f"{LIB_PATH} has ABI version {L.csrspmm_b200_abi_version()}, expected {ABI_VERSION}")

@@ -8,6 +8,8 @@
 // Every entry is one sum in a fixed order: no atomics.
 #pragma once
 
+#include <climits>
+
 #include "common.cuh"
 #include "score_types.cuh"
 
@@ -193,6 +195,72 @@ __global__ void __launch_bounds__(kSddmmThreads) sddmm_kernel(SddmmParams p)
             if (i < end && gl == 0) p.out[begin + i] = p.alpha * sum;
         }
     }
+}
+
+// ---- the gradient for B of a small product -----------------------------------------------------------------
+//
+// C = alpha * A^T * G without a transpose: a warp owns a row of C (a column of A) and up to 32 * kTransposedVectors vectors of its columns, looks
+// through all of A's columns and adds up the entries that are its own, in stored order.  That reads nnz columns Kd times, and takes one
+// launch where transposition and product take seven: what a small training step costs is those launches.
+
+constexpr int kTransposedThreads = 256;
+constexpr int kTransposedVectors = 4;
+
+struct TransposedParams {
+    int M, Kd, nvec, nnz;
+    const int* row_ptr;
+    const int* col_idx;
+    const float* values;
+    const float* G;
+    long long ldg;
+    float alpha;
+    float* C;
+    long long ldc;
+};
+
+template <int VW>
+__global__ void __launch_bounds__(kTransposedThreads) spmm_transposed_kernel(TransposedParams p)
+{
+    constexpr int NV = kTransposedVectors, U = 4;
+    wait_for_previous_grid();
+    const int lane = threadIdx.x & 31;
+    const long long own = (long long)blockIdx.x * (kTransposedThreads / 32) + (threadIdx.x >> 5);  // row of C and part of its columns
+    const int parts = (p.nvec + 32 * NV - 1) / (32 * NV);
+    const int row = (int)(own / parts), v0 = (int)(own % parts) * 32 * NV + lane;
+    if (row >= p.Kd) return;
+    Vec<VW> sum[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) sum[k].zero();
+    for (int base = 0; base < p.nnz; base += 32 * U) {
+        int col[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long e = (long long)base + u * 32 + lane;
+            col[u] = e < p.nnz ? min(max(__ldg(p.col_idx + e), 0), p.Kd - 1) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            unsigned mine = __ballot_sync(kAllLanes, col[u] == row);
+            for (; mine != 0; mine &= mine - 1) {
+                const int e = base + u * 32 + __ffs(mine) - 1;
+                const float* from = p.G + (long long)row_of_entry(p.row_ptr, p.M, e, lane) * p.ldg;
+                const float value = __ldg(p.values + e);
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    if (v0 + k * 32 < p.nvec) {
+                        Vec<VW> g;
+                        g.load_nc(from + (long long)(v0 + k * 32) * VW);
+                        sum[k].fma(value, g);
+                    }
+                }
+            }
+        }
+        if (base > INT_MAX - 32 * U) break;
+    }
+    float* const to = p.C + (long long)row * p.ldc;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+        if (v0 + k * 32 < p.nvec) sum[k].epilogue0(p.alpha).store(to + (long long)(v0 + k * 32) * VW);
 }
 
 }  // namespace csrspmm_b200

@@ -820,6 +820,8 @@ void init_scores(PyObject* addresses)
     fill(g_scores.route, addresses, "route");
     fill(g_scores.route_backward, addresses, "route_backward");
     fill(g_scores.sddmm, addresses, "sddmm");
+    fill(g_scores.transposed_pays, addresses, "spmm_transposed_pays");
+    fill(g_scores.transposed, addresses, "spmm_transposed");
     fill(g_scores.distill, addresses, "distill");
     fill(g_scores.distill_backward, addresses, "distill_backward");
     fill(g_scores.distill_grad, addresses, "distill_grad");

@@ -10,6 +10,9 @@ struct ScoreLibrary {
     int (*route_backward)(const csrspmm_b200_route_args*, const int32_t*, const float*, const float*, int64_t, void*, int64_t, csrspmm_b200_stream_t);
     int (*sddmm)(int32_t, int32_t, int32_t, int64_t, const int32_t*, const int32_t*, const float*, int64_t, const float*, int64_t, float, float*,
                  csrspmm_b200_stream_t);
+    int (*transposed_pays)(int32_t, int32_t, int64_t);
+    int (*transposed)(int32_t, int32_t, int32_t, int64_t, const int32_t*, const int32_t*, const float*, const float*, int64_t, float, float*, int64_t,
+                      csrspmm_b200_stream_t);
     int (*distill)(const csrspmm_b200_distill_args*, float*, float*, csrspmm_b200_stream_t);
     int (*distill_backward)(const csrspmm_b200_distill_args*, const float*, const float*, int64_t, void*, int64_t, csrspmm_b200_stream_t);
     int (*distill_grad)(const csrspmm_b200_distill_args*, const float*, int64_t, float*, void*, int64_t, csrspmm_b200_stream_t);
@@ -252,6 +255,43 @@ at::Tensor call_sddmm(const at::Tensor& rp, const at::Tensor& ci, const at::Tens
     return op.call(rp, ci, G, B, alpha);
 }
 
+// alpha * A^T * G: in one launch where the matrix is small, else by its transpose
+at::Tensor op_spmm_transposed(const at::Tensor& rp, const at::Tensor& ci, const at::Tensor& va, const at::Tensor& G, c10::SymInt rows, double alpha)
+{
+    return as_operator([&] {
+        const int64_t Kd = rows.expect_int();
+        check_csr(rp, ci, va, G, false);
+        want(va.size(0) == ci.size(0), "values and col_idx differ in length");
+        want(G.size(0) == rp.size(0) - 1, "G must have a row for each row of the matrix");
+        const int32_t Nd = as_int32(G.size(1), "G has too many columns"), M = as_int32(G.size(0), "too many rows");
+        if (!g_scores.transposed_pays(as_int32(Kd, "too many columns"), Nd, ci.size(0))) {
+            Product q;
+            std::tie(q.rp, q.ci, q.va) = transpose(rp, ci, va, Kd);
+            q.B = G;
+            q.alpha = alpha;
+            return run_product(q);
+        }
+        want(ci.size(0) == 0 || (M > 0 && Kd > 0), "entries, but no rows or columns");
+        const c10::cuda::CUDAGuard guard(G.device());
+        at::Tensor C = at::detail::empty_cuda({Kd, G.size(1)}, at::kFloat, G.device(), std::nullopt);
+        int status;
+        {
+            const WithoutGil nogil;
+            status = g_scores.transposed(M, static_cast<int32_t>(Kd), Nd, ci.size(0), address<int32_t>(rp), address<int32_t>(ci), address<float>(va),
+                                         address<float>(G), leading(G), static_cast<float>(alpha), address<float>(C), G.size(1),
+                                         current_stream(G.device()));
+        }
+        check(status, "csrspmm_b200_spmm_transposed");
+        return C;
+    });
+}
+
+at::Tensor call_spmm_transposed(const at::Tensor& rp, const at::Tensor& ci, const at::Tensor& va, const at::Tensor& G, c10::SymInt rows, double alpha)
+{
+    static const auto op = dispatched<decltype(op_spmm_transposed)>("csrspmm_b200::spmm_transposed");
+    return op.call(rp, ci, va, G, rows, alpha);
+}
+
 at::Tensor op_weighted_spmm(const at::Tensor& rp, const at::Tensor& ci, const at::Tensor& va, const at::Tensor& B, double alpha)
 {
     return op_spmm(rp, ci, va, B, alpha, "auto");
@@ -283,10 +323,7 @@ struct WeightedSpmm : torch::autograd::Function<WeightedSpmm> {
         const double alpha = ctx->saved_data["alpha"].toDouble();
         const at::Tensor G = grads[0].contiguous();
         if (ctx->needs_input_grad(2)) out[2] = call_sddmm(saved[0], saved[1], G, saved[3], alpha);
-        if (ctx->needs_input_grad(3)) {
-            const auto t = call_transpose(saved[0], saved[1], saved[2], ctx->saved_data["Kd"].toSymInt());
-            out[3] = call_spmm(std::get<0>(t), std::get<1>(t), std::get<2>(t), G, alpha, "auto");
-        }
+        if (ctx->needs_input_grad(3)) out[3] = call_spmm_transposed(saved[0], saved[1], saved[2], G, ctx->saved_data["Kd"].toSymInt(), alpha);
         return out;
     }
 };
@@ -501,6 +538,7 @@ TORCH_LIBRARY_IMPL(csrspmm_b200, CUDA, scores)
     scores.impl("route", op_route);
     scores.impl("route_backward", op_route_backward);
     scores.impl("sddmm", op_sddmm);
+    scores.impl("spmm_transposed", op_spmm_transposed);
     scores.impl("weighted_spmm", op_weighted_spmm);
     scores.impl("distill_loss", op_distill_loss);
     scores.impl("distill_with_stats", op_distill_with_stats);

@@ -54,12 +54,14 @@ _library.define("spmm_(Tensor row_ptr, Tensor col_idx, Tensor values, Tensor B, 
 _library.define("transpose(Tensor row_ptr, Tensor col_idx, Tensor values, SymInt Kd) -> (Tensor, Tensor, Tensor)",
                 tags=(torch.Tag.pt2_compliant_tag,))
 # Routing, the gradient for a matrix's stored values, distillation (csrc/torch/scores.h).  route, weighted_spmm and distill_loss
-# have gradients; *_backward and distill_with_stats are what those are made of.
+# have gradients; *_backward, spmm_transposed and distill_with_stats are what those are made of.
 _library.define("route(Tensor logits, int k, Tensor? bias, str score, int groups, int top_groups, int group_top, bool renormalize, float scale) "
                 "-> (Tensor, Tensor, Tensor)", tags=(torch.Tag.pt2_compliant_tag,))
 _library.define("route_backward(Tensor grad, Tensor logits, Tensor col_idx, Tensor values, int k, str score, bool renormalize, float scale) "
                 "-> Tensor", tags=(torch.Tag.pt2_compliant_tag,))
 _library.define("sddmm(Tensor row_ptr, Tensor col_idx, Tensor G, Tensor B, float alpha) -> Tensor", tags=(torch.Tag.pt2_compliant_tag,))
+_library.define("spmm_transposed(Tensor row_ptr, Tensor col_idx, Tensor values, Tensor G, SymInt rows, float alpha) -> Tensor",
+                tags=(torch.Tag.pt2_compliant_tag,))
 _library.define("weighted_spmm(Tensor row_ptr, Tensor col_idx, Tensor values, Tensor B, float alpha) -> Tensor",
                 tags=(torch.Tag.pt2_compliant_tag,))
 _library.define("distill_loss(Tensor logits, Tensor row_ptr, Tensor col_idx, Tensor values, float temperature, bool log_probs) -> Tensor",
@@ -102,6 +104,11 @@ def _route_backward_fake(grad, logits, col_idx, values, k, score, renormalize, s
 @torch.library.register_fake("csrspmm_b200::sddmm")
 def _sddmm_fake(row_ptr, col_idx, G, B, alpha):
     return G.new_empty(col_idx.shape)
+
+
+@torch.library.register_fake("csrspmm_b200::spmm_transposed")
+def _spmm_transposed_fake(row_ptr, col_idx, values, G, rows, alpha):
+    return G.new_empty((rows, G.shape[1]))
 
 
 @torch.library.register_fake("csrspmm_b200::weighted_spmm")

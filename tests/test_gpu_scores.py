@@ -346,6 +346,40 @@ def test_weighted_spmm_and_its_gradients(cuda_lib, Nd):
     assert abs((f(step) - f(-step)) / (2 * step) - float((grad * way.double()).sum())) <= 1e-3 * float((grad * way.double()).abs().sum())
 
 
+@pytest.mark.parametrize("Nd", [1, 2, 6, 24, 130, 512, 515, 1024, 2050])
+def test_small_product_with_the_transpose(cuda_lib, Nd):
+    rp, ci, va = _csr(150, 70, torch.randint(0, 6, (150,), generator=torch.Generator().manual_seed(Nd)), 17)
+    ci[3], ci[9] = 70, -4  # the nearest inside, as in a product
+    wide = torch.randn(150, Nd + 3, device="cuda", generator=_gen(18))
+    for G in (wide[:, :Nd], wide[:, 1 : Nd + 1], wide[:, :Nd].contiguous()):
+        got = torch.ops.csrspmm_b200.spmm_transposed(rp, ci, va, G, 70, -0.5)
+        terms = va.double()[:, None] * G.double()[_rows(rp)]
+        index = ci.long().clamp(0, 69)
+        want = torch.zeros(70, Nd, dtype=torch.float64, device="cuda").index_add(0, index, terms)
+        most = int(torch.bincount(index).max())
+        bound = (most + 1) * U * 0.5 * torch.zeros_like(want).index_add(0, index, terms.abs())  # a sum in turn and the factor
+        assert got.shape == want.shape and ((got.double() + 0.5 * want).abs() <= bound + 1e-38).all()
+        assert torch.equal(got, torch.ops.csrspmm_b200.spmm_transposed(rp, ci, va, G, 70, -0.5))
+    none = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, device="cuda")
+    assert (torch.ops.csrspmm_b200.spmm_transposed(*none, wide[:3], 5, 1.0) == 0).all()
+    assert torch.ops.csrspmm_b200.spmm_transposed(*none, wide[:3], 0, 1.0).shape == (0, Nd + 3)
+
+
+def test_both_ways_to_the_gradient_of_b_agree(cuda_lib):
+    from csrspmm_b200 import _lib
+    pays = _lib.lib().csrspmm_b200_spmm_transposed_pays
+    for M, Kd, Nd, mean in ((300, 200, 64, 4), (5000, 4000, 48, 9)):
+        rp, ci, va = _csr(M, Kd, [mean] * M, 19)
+        G = torch.randn(M, Nd, device="cuda", generator=_gen(20))
+        assert bool(pays(Kd, Nd, ci.numel())) == (M == 300)
+        got = torch.ops.csrspmm_b200.spmm_transposed(rp, ci, va, G, Kd, 1.5)
+        t = TL.transpose_csr(rp, ci, va, Kd)
+        assert torch.allclose(got, torch.ops.csrspmm_b200.spmm(*t, G, 1.5, "auto"), rtol=1e-4, atol=1e-4)
+        B = torch.randn(Kd, Nd, device="cuda", generator=_gen(21), requires_grad=True)
+        (dB,) = torch.autograd.grad(ops.weighted_spmm(rp, ci, va, B, 1.5), B, G)
+        assert torch.equal(dB, got)
+
+
 # ---- distillation ------------------------------------------------------------------------------------------------
 
 def distill_f64(x, rp, ci, va, g, t=1.0, log_probs=False):
@@ -817,6 +851,7 @@ def test_registration(cuda_lib):
         torch.library.opcheck(O.distill_loss, (leaf, rp, ci, va, 2.0, False), **how)
         torch.library.opcheck(O.weighted_spmm, (rp, ci, va, torch.randn(16, 5, device="cuda", requires_grad=leaf.requires_grad), 1.0), **how)
     torch.library.opcheck(O.sddmm, (rp, ci, torch.randn(6, 5, device="cuda"), torch.randn(16, 5, device="cuda"), 1.0), **how)
+    torch.library.opcheck(O.spmm_transposed, (rp, ci, va, torch.randn(6, 5, device="cuda"), 16, 1.0), **how)
     torch.library.opcheck(O.route_backward, (va, x, ci, va, 4, "softmax", False, 1.0), **how)
     torch.library.opcheck(O.distill_loss_grad, (x, rp, ci, va, torch.ones(6, device="cuda"), 1.0, False), **how)
     loss, stats = O.distill_with_stats(x, rp, ci, va, 1.0, False)

@@ -69,6 +69,18 @@ def test_bad_sizes_of_the_sampled_product_are_refused(args):
     assert _lib.lib().csrspmm_b200_sddmm(*args, P, P, P, 4, P, 4, 1.0, P, None) == _lib.ERR_BAD_ARG
 
 
+def test_bad_arguments_of_the_small_product_with_the_transpose_are_refused():
+    L = _lib.lib()
+    good = [4, 4, 4, 5, P, P, P, P, 4, 1.0, P, 4, None]
+    for at, value in ((0, -1), (1, -1), (2, -1), (3, -1), (3, 1 << 31), (0, 0), (4, None), (5, None), (6, None), (7, None), (8, 3), (10, None), (11, 3)):
+        args = list(good)
+        args[at] = value
+        assert L.csrspmm_b200_spmm_transposed(*args) == _lib.ERR_BAD_ARG, (at, value)
+    assert L.csrspmm_b200_spmm_transposed(0, 0, 4, 0, None, None, None, None, 4, 1.0, None, 4, None) == 0
+    assert L.csrspmm_b200_spmm_transposed_pays(100, 64, 500) == 1 and L.csrspmm_b200_spmm_transposed_pays(1 << 20, 64, 1 << 24) == 0
+    assert L.csrspmm_b200_spmm_transposed_pays(-1, 64, 500) == 0
+
+
 def test_bad_pointers_of_the_sampled_product_are_refused():
     good = [4, 4, 4, 5, P, P, P, 4, P, 4, 1.0, P, None]
     for at, value in ((4, None), (5, None), (6, None), (7, 3), (8, None), (9, 3), (11, None)):
@@ -137,7 +149,7 @@ def fake():
     for name in ("fake_kernels", "fake_launched"):
         getattr(L, name).restype = C.c_size_t
     L.fake_reset.argtypes = [C.c_long]
-    for name in ("route", "route_backward", "sddmm", "distill", "distill_backward", "distill_grad"):
+    for name in ("route", "route_backward", "sddmm", "spmm_transposed", "distill", "distill_backward", "distill_grad"):
         getattr(L, "csrspmm_b200_" + name).argtypes = getattr(_lib.lib(), "csrspmm_b200_" + name).argtypes
     return L
 
@@ -164,7 +176,8 @@ def test_nothing_is_compiled_that_no_call_launches(fake):
                 assert fake.csrspmm_b200_distill_backward(C.byref(d), P, P, 1, P, V, None) == 0
     for Nd in (1, 2, 3, 8, 9, 16, 17, 18, 33, 34, 50, 64, 65, 90, 100, 129, 130, 200, 256, 257, 258, 512, 513, 514, 1000, 1024):
         assert fake.csrspmm_b200_sddmm(100, 50, Nd, 1000, P, P, P, Nd, P, Nd, 1.0, P, None) == 0
-    every = {k for k in _names(fake.fake_kernels) if any(w in k for w in ("route_", "sddmm_", "distill_"))}
+        assert fake.csrspmm_b200_spmm_transposed(100, 50, Nd, 1000, P, P, P, P, Nd, 1.0, P, Nd, None) == 0
+    every = {k for k in _names(fake.fake_kernels) if any(w in k for w in ("route_", "sddmm_", "distill_", "spmm_transposed"))}
     assert every and sorted(every - _names(fake.fake_launched)) == []
 
 
@@ -174,6 +187,7 @@ def test_a_failed_launch_is_reported(fake):
                 lambda: fake.csrspmm_b200_route(C.byref(_route(E=1024, ld=1024)), P, P, P, None),
                 lambda: fake.csrspmm_b200_route(C.byref(_route(T=0)), C.addressof(C.create_string_buffer(16)), P, P, None),
                 lambda: fake.csrspmm_b200_sddmm(4, 4, 4, 5, P, P, P, 4, P, 4, 1.0, P, None),
+                lambda: fake.csrspmm_b200_spmm_transposed(4, 4, 4, 5, P, P, P, P, 4, 1.0, P, 4, None),
                 lambda: fake.csrspmm_b200_distill(C.byref(_distill()), P, P, None),
                 lambda: fake.csrspmm_b200_distill_backward(C.byref(_distill()), P, P, 1, P, 100, None),
                 lambda: fake.csrspmm_b200_distill_grad(C.byref(_distill()), P, 1, P, P, 100, None)):
