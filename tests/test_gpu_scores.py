@@ -856,3 +856,18 @@ def test_registration(cuda_lib):
     torch.library.opcheck(O.distill_loss_grad, (x, rp, ci, va, torch.ones(6, device="cuda"), 1.0, False), **how)
     loss, stats = O.distill_with_stats(x, rp, ci, va, 1.0, False)
     torch.library.opcheck(O.distill_backward, (loss, x, rp, ci, va, stats, 1.0, False), **how)
+
+
+def test_the_operators_and_their_gradients_trace(cuda_lib):
+    O = torch.ops.csrspmm_b200
+    x, B = (torch.randn(*shape, device="cuda", generator=_gen(80), requires_grad=True) for shape in ((16, 64), (64, 24)))
+    slots = torch.randperm(64, device="cuda", generator=_gen(81)).int()
+    rp_t, ci_t, va_t = teacher(16, 24, [4] * 16, 82)
+
+    def loss(x, B):
+        rp, ci, va = O.route(x, 4, None, "sigmoid", 1, 1, 1, True, 1.0)
+        return O.distill_loss(O.weighted_spmm(rp, slots, va, B, 1.0), rp_t, ci_t, va_t, 1.0, False).mean()
+
+    want = torch.autograd.grad(loss(x, B), (x, B))
+    got = torch.autograd.grad(torch.compile(loss, backend="aot_eager", fullgraph=True)(x, B), (x, B))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
