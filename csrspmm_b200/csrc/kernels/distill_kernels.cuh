@@ -14,8 +14,9 @@
 // warp's (distill_short_kernel); rows that are longer than a cluster's shared memory are read twice (distill_long_kernel).
 //
 // Sums, maxima and the loss are fp32.  Exponentials are 2^y with y = x c - m c, c = log2(e) / t, m a maximum: one fused multiply-add each.  The
-// product m c is rounded once and the same rounded one serves the sum, the loss and the gradient, so that its rounding cancels.  Where m c
-// overflows (a row of the type's lowest) y = (x - m) c.
+// product m c is rounded once and the same rounded one serves the sum, the loss and the gradient, so that its rounding cancels.  That holds
+// while its rounding is small as an exponent: from |m c| = 2^24 on, where it passes a half (a row of a mask such as -1e30; beyond 2^31 it alone
+// would overflow 2^y), y = (x - m) c.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -65,6 +66,8 @@ __device__ __forceinline__ Pair exp2_approx(Pair v)
     return pair_of(exp2_approx(w.x), exp2_approx(w.y));
 }
 
+constexpr float kFarProduct = 16777216.0f;  // 2^24: below it a product is off by at most a half
+
 // y above, for one maximum
 struct Exponent {
     float m, mc, c;
@@ -74,7 +77,7 @@ struct Exponent {
         m = top;
         c = scale;
         mc = __fmul_rn(top, scale);
-        far = !(fabsf(mc) <= -kLowest);
+        far = !(fabsf(mc) < kFarProduct);
     }
     template <bool FAR>
     __device__ __forceinline__ float of(float x) const
@@ -92,8 +95,15 @@ struct Exponent {
             return fma2(x, pair_of(c, c), pair_of(-mc, -mc));
         }
     }
-    // of a smaller maximum, whose own product was rounded too
-    __device__ __forceinline__ float of_max(float other) const { return far ? (other - m) * c : __fsub_rn(__fmul_rn(other, c), mc); }
+    // what y is too large by: the rounding of m c
+    __device__ __forceinline__ float excess() const { return far ? 0.0f : __fmaf_rn(m, c, -mc); }
+    // of a smaller maximum, to which its own sum was taken: with the rounding of its product too, or without where that one is far
+    __device__ __forceinline__ float of_max(float other) const
+    {
+        const Exponent o(other, c);
+        if (!far && !o.far) return __fsub_rn(o.mc, mc);
+        return (other - m) * c + (excess() - o.excess());
+    }
 };
 
 // A maximum and the sum of 2^y relative to it; none: kLowest and 0.
