@@ -32,12 +32,16 @@ struct SddmmParams {
     float* out;
 };
 
+// Steps of 32 that cover `rows` rows, of which there may be 2^31 - 1.
+__host__ __device__ constexpr int search_step(int rows) { return (rows - 1) / 32 + 1; }
+static_assert(search_step(2) == 1 && search_step(33) == 2 && search_step(INT_MAX) == 1 << 26, "whole steps, without passing 32 bits");
+
 // The last row r of [0, M) with row_ptr[r] <= e (0 where there is none), by all lanes of a warp.
 __device__ __forceinline__ int row_of_entry(const int* row_ptr, int M, int e, int lane)
 {
     int lo = 0, hi = M;  // the answer is in [lo, hi)
     while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32;
+        const int step = search_step(hi - lo);
         const long long at = lo + (long long)lane * step;
         const bool at_or_before = at < hi && (lane == 0 || __ldg(row_ptr + at) <= e);
         const int last = 31 - __clz(__ballot_sync(kAllLanes, at_or_before));
@@ -96,9 +100,9 @@ __global__ void __launch_bounds__(kSddmmThreads) sddmm_kernel(SddmmParams p)
     for (int i = tid; i < kSddmmMostEntries; i += kSddmmThreads) row_of[i] = 0;
     __syncthreads();
     const int r0 = bounds[0], r1 = bounds[1];
-    for (int r = r0 + 1 + tid; r <= r1; r += kSddmmThreads) {  // where the rows after the first begin; of empty ones the last counts
+    for (long long r = r0 + 1LL + tid; r <= r1; r += kSddmmThreads) {  // where the rows after the first begin; of empty ones the last counts
         const long long at = (long long)__ldg(p.row_ptr + r) - begin;
-        if (at >= 0 && at < n) atomicMax(&row_of[at], r - r0);
+        if (at >= 0 && at < n) atomicMax(&row_of[at], (int)(r - r0));
     }
     __syncthreads();
     {  // running maximum over the run, kEach entries a thread

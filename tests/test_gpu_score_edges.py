@@ -3,6 +3,7 @@ out.  Against the definitions in 64 bits and the tolerances of test_gpu_scores."
 import pytest
 import torch
 
+from csrspmm_b200 import ops
 from test_gpu_scores import _gen, check_distill, teacher
 
 pytestmark = pytest.mark.gpu
@@ -37,3 +38,17 @@ def test_distill_of_rows_about_where_the_exponent_is_taken_another_way(cuda_lib,
     x[:, : V // 3] -= 12.0
     x[1, V // 2 :] -= 7.0
     check_distill(x + sign * 11629080.0, *teacher(4, V, [6] * 4, 5))
+
+
+def test_the_gradients_of_a_matrix_of_nearly_2_to_31_rows(cuda_lib):
+    M, Kd = 2 ** 31 - 2, 5
+    rp = torch.zeros(M + 1, dtype=torch.int32, device="cuda")
+    rp[M - 2] = 2  # two entries in row M - 3, none in M - 2, one in M - 1
+    rp[M - 1] = 2
+    rp[M] = 3
+    ci = torch.tensor([4, 0, 4], dtype=torch.int32, device="cuda")
+    va = torch.tensor([2.0, 3.0, 5.0], device="cuda")
+    G, B = torch.zeros(M, 1, device="cuda"), torch.tensor([[1.0], [0.0], [0.0], [0.0], [7.0]], device="cuda")
+    G[M - 3], G[M - 1] = 11.0, 13.0
+    assert ops.sddmm(rp, ci, G, B).tolist() == [77.0, 11.0, 91.0]
+    assert torch.ops.csrspmm_b200.spmm_transposed(rp, ci, va, G, Kd, 1.0).flatten().tolist() == [33.0, 0.0, 0.0, 0.0, 87.0]
