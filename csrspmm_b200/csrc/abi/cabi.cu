@@ -56,11 +56,7 @@ void fill_params(const csrspmm_b200_args* a, const Plan& plan, SpmmParams* out)
     p.alpha = a->alpha;
     p.beta = a->beta;
     p.status_word = a->status_word;
-    // CSRSPMM_TEST_WAIT_LIMIT=<n> (tests only): a wait on a row copy gives up after n attempts, so the
-    // give-up path can be exercised without anything being stuck (the drain wait keeps the full limit)
-    p.wait_limit = kWaitSpinLimit;
-    if (const char* e = std::getenv("CSRSPMM_TEST_WAIT_LIMIT"))
-        if (*e != 0) p.wait_limit = (unsigned)std::strtoul(e, nullptr, 10);
+    p.wait_limit = wait_limit(kWaitSpinLimit);
     *out = p;
 }
 

@@ -127,6 +127,7 @@ cudaError_t launch_loss(const csrspmm_b200_distill_args* a, DistillParams p, cud
         });
     p.slot_bytes = (int)slot;
     p.ring_offset = (int)before;
+    p.wait_limit = wait_limit(kWaitSpinLimit);
     return for_type(a->logit_type, [&](auto zero) {
         using T = decltype(zero);
         if (p.slot_bytes <= kFewBytes) return launch_ring<T, 128, GRADIENT>(a, p, 6, st);

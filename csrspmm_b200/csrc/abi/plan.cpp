@@ -14,6 +14,12 @@ thread_local char g_last_error[512] = "";
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 }  // namespace
 
+unsigned wait_limit(unsigned usual)
+{
+    const char* e = std::getenv("CSRSPMM_TEST_WAIT_LIMIT");
+    return e != nullptr && *e != 0 ? (unsigned)std::strtoul(e, nullptr, 10) : usual;
+}
+
 void set_last_error(const char* fmt, ...)
 {
     va_list ap;

@@ -87,6 +87,10 @@ size_t worst_case_workspace(const csrspmm_b200_args* a);
 // Below 250 MB of gather the launch costs more than it gives (50 columns, 220 MB 45.6 and 45.9).
 size_t padded_b_bytes(const csrspmm_b200_args* a);
 
+// Attempts of a wait for a copy: `usual`, or CSRSPMM_TEST_WAIT_LIMIT=<n> (tests only), so that the path of a wait that runs out can be
+// exercised without anything being stuck (the waits for copies in flight before a CTA ends keep the full limit).
+unsigned wait_limit(unsigned usual);
+
 void set_last_error(const char* fmt, ...);
 const char* get_last_error();
 

@@ -51,6 +51,7 @@ struct DistillParams {
     int log_parts, per;  // a row is cut into 2^log_parts runs of `per` columns, a multiple of 64
     // the ring kernel's: rows of a CTA or cluster, copies on their way and the room of each, the shared memory before them
     int rows, slots, slot_bytes, ring_offset;
+    unsigned wait_limit;  // attempts of a wait for a copy
 };
 
 __device__ __forceinline__ float exp2_approx(float v)
@@ -552,13 +553,17 @@ __global__ void __launch_bounds__(kShortThreads) distill_short_kernel(DistillPar
 
 constexpr int kListed = 256;  // entries of a row that are kept in shared memory; rows with more read them where they need them
 constexpr int kMostSlots = 2;
-// Attempts of a wait for the other parts of a row, which may still be at the row before: one of many entries that name columns twice
-// takes its manager the square of their number.
-constexpr unsigned kToldLimit = 64 * kWaitSpinLimit;
+// How much longer than a copy takes may be waited for what a manager does first, who may still walk over the entries of the row before.
+constexpr unsigned kWalkFactor = 64;
+constexpr unsigned kToldLimit = kWalkFactor * kWaitSpinLimit;
+
+// From so many entries on the copy of a later row is asked for before the walk that writes the entries' columns, which then reads its logits from
+// memory: the workers wait for a copy, not for the walk.
+constexpr int kLongWalk = 2048;
 
 struct RingRow {  // what the workers need to write a part of dx
     float m, scale;
-    int zero, aligned;
+    int zero, aligned, vectors;
     void* to;
 };
 
@@ -576,7 +581,7 @@ struct RingShared {
     int col[3][kListed];
     alignas(8) unsigned long long full[kMostSlots];  // a slot's copies have arrived
     alignas(8) unsigned long long told[2];           // the blocks of a row have
-    int dead;                                        // something did not within the limit: every row from there on is NaN
+    int dead;                                        // something did not within the limit: from there on the loss and gradient of every row are NaN
     int joined;                                      // rows whose sums the manager has taken
 };
 
@@ -633,12 +638,12 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
         for (int i = 0; i < rows; ++i) {
             bool arrived = *dead == 0;
             if (arrived) {
-                arrived = mbar_wait_bounded(smem_u32(&sh.full[slot]), phase);
+                arrived = mbar_wait_bounded(smem_u32(&sh.full[slot]), phase, kWalkFactor * p.wait_limit);
                 if (!arrived) *dead = 1;
             }
             if (!arrived) {  // without copies to wait for, no further ahead of the manager than they would let this warp be
                 volatile int* const joined = &sh.joined;
-                for (unsigned spin = 0; spin < kWaitSpinLimit && *joined + p.slots <= i; ++spin) {}
+                for (unsigned spin = 0; spin < kToldLimit && *joined + p.slots <= i; ++spin) {}
             }
             __syncwarp();
             const uint4* const from = reinterpret_cast<const uint4*>(ring + slot * p.slot_bytes);
@@ -677,8 +682,9 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
                 barrier_sync(kRow + slot, ALL);
                 const RingRow row = sh.row[slot];
                 T* const to = static_cast<T*>(row.to);
-                if (row.zero) {
-                    for (int k = tid; k < vectors; k += WORKERS) store_vector(to + (long long)k * N, make_uint4(0, 0, 0, 0), row.aligned);
+                if (row.zero || !arrived) {
+                    const unsigned word = row.zero ? 0u : Words<T>::kNaN;
+                    for (int k = tid; k < row.vectors; k += WORKERS) store_vector(to + (long long)k * N, make_uint4(word, word, word, word), row.aligned);
                 } else {
                     const Exponent z(row.m, c);
                     const auto write = [&](auto far) {
@@ -697,7 +703,9 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
     } else {  // ---- the manager
         const int rank = (int)blockIdx.x & (parts - 1);
         const T* const all_x = static_cast<const T*>(p.x);
+        int issued = 0;
         const auto issue = [&](int i, int slot) {  // the copies of row first_row + i
+            ++issued;
             const Place at(p, first_row + i);
             const T* x = all_x + (long long)at.row * p.ldx;
             const Part<T> part(x, at.c0, at.c1);
@@ -775,9 +783,10 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
             const T* x = all_x + (long long)at.row * p.ldx;
             const Part<T> part(x, at.c0, at.c1);
             const T* const here = reinterpret_cast<const T*>(ring + slot * p.slot_bytes);
+            bool held = true;                            // the slot is still this row's
             const auto element = [&](int col) {  // of this part
                 const int k = col - part.first;
-                return to_f32(k >= 0 && k < part.vectors * N ? here[k] : x[col]);
+                return to_f32(held && k >= 0 && k < part.vectors * N ? here[k] : x[col]);
             };
             const Teacher t = next;
             const bool listed = t.count <= kListed, counts = t.top != -CUDART_INF_F;
@@ -789,7 +798,7 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
             // elements of the lanes.
             bool arrived = *dead == 0;
             if (arrived) {
-                arrived = mbar_wait_bounded(smem_u32(&sh.full[slot]), phase);
+                arrived = mbar_wait_bounded(smem_u32(&sh.full[slot]), phase, p.wait_limit);
                 if (!arrived) *dead = 1;
             }
             arrived = __all_sync(kAllLanes, arrived);
@@ -820,7 +829,8 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
             if (lane == 0) *const_cast<volatile int*>(&sh.joined) = i + 1;
             constexpr int kJoined = W < 16 ? 16 : 32;
             const int whose = lane % kJoined;
-            const MaxSum mine = join_lanes<kJoined>(whose < W ? sh.part[slot][whose] : whose == W ? edges : MaxSum{kLowest, 0.0f}, c);
+            MaxSum mine = join_lanes<kJoined>(whose < W ? sh.part[slot][whose] : whose == W ? edges : MaxSum{kLowest, 0.0f}, c);
+            if (!arrived) mine.s = CUDART_NAN_F;
             if (share != 0.0f) cross -= Exponent(mine.m, c).of_max(top) * CUDART_LN2_F * share;
             if constexpr (!GRADIENT) {
                 if (arrived && i + p.slots < rows) {  // everybody has read the slot
@@ -849,7 +859,7 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
             const float scale = weight * p.temperature * mass / all.s;
             if constexpr (GRADIENT) {
                 T* const to = static_cast<T*>(p.dx) + (long long)at.row * p.ldd + part.first;
-                if (lane == 0) sh.row[slot] = {all.m, scale, zero, (reinterpret_cast<uintptr_t>(to) & 15u) == 0, to};
+                if (lane == 0) sh.row[slot] = {all.m, scale, zero, (reinterpret_cast<uintptr_t>(to) & 15u) == 0, part.vectors, to};
                 barrier_arrive(kRow + slot, ALL);
             }
 
@@ -893,6 +903,12 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
                         if (inside(column(j))) named[(column(j) - at.c0) >> 5] = 0;
                 }
                 const bool ready = listed && !repeats;  // what becomes of the entries' columns is known before the workers are done
+                const auto next_copy = [&] {
+                    if (arrived && i + p.slots < rows) {  // everybody has read the slot
+                        if (lane == 0) fence_proxy_async_smem();
+                        issue(i + p.slots, slot);
+                    }
+                };
                 if (ready) {
                     for (int j = lane; j < t.count; j += 32)
                         if (inside(column(j))) sh.v[i % 3][j] = gradient(column(j), share_of(j));
@@ -900,6 +916,10 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
                 if (i + 1 < rows) next = teach(i + 1, offsets[1], offsets[2]);
                 barrier_sync(kWritten + slot, ALL);  // what the workers wrote comes before what is written here
                 if (!ready) {
+                    if (repeats || t.count > kLongWalk) {
+                        held = false;
+                        next_copy();
+                    }
                     for (int j = lane; j < t.count; j += 32) {
                         const int col = column(j);
                         if (!inside(col)) continue;
@@ -915,10 +935,7 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
                     }
                     __syncwarp();
                 }
-                if (arrived && i + p.slots < rows) {  // everybody has read the slot
-                    if (lane == 0) fence_proxy_async_smem();
-                    issue(i + p.slots, slot);
-                }
+                if (held) next_copy();
                 if (ready) {
                     for (int j = lane; j < t.count; j += 32)
                         if (inside(column(j))) out[column(j)] = from_f32<T>(sh.v[i % 3][j]);
@@ -932,11 +949,8 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
             if (++slot == p.slots) slot = 0, phase ^= 1;
         }
         async_wait<0>();
-        if (*dead != 0 && lane == 0) {  // no copy may arrive after the CTA has gone: each barrier is at the phase of its last one, or past it
-            for (int k = 0; k < p.slots; ++k) {
-                mbar_wait_bounded(smem_u32(&sh.full[k]), 0);
-                mbar_wait_bounded(smem_u32(&sh.full[k]), 1);
-            }
+        if (*dead != 0 && lane == 0) {  // no copy may arrive after the CTA has gone
+            for (int i = max(issued - p.slots, 0); i < issued; ++i) mbar_wait_bounded(smem_u32(&sh.full[i % p.slots]), (unsigned)(i / p.slots) & 1u);
         }
     }
     if (parts > 1) cooperative_groups::this_cluster().sync();  // nobody leaves while another may still tell it something

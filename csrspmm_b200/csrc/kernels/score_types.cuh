@@ -89,7 +89,7 @@ template <class T>
 struct Words;
 template <>
 struct Words<float> {
-    static constexpr unsigned kMinusInf = 0xff800000u;
+    static constexpr unsigned kMinusInf = 0xff800000u, kNaN = 0x7fffffffu;
     static __device__ __forceinline__ unsigned max(unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
     static __device__ __forceinline__ float largest(unsigned a) { return __uint_as_float(a); }
     template <class F>
@@ -152,11 +152,11 @@ struct HalfWords {
 };
 template <>
 struct Words<__nv_bfloat16> : HalfWords<__nv_bfloat16, __nv_bfloat162> {
-    static constexpr unsigned kMinusInf = 0xff80ff80u;
+    static constexpr unsigned kMinusInf = 0xff80ff80u, kNaN = 0x7fff7fffu;
 };
 template <>
 struct Words<__half> : HalfWords<__half, __half2> {
-    static constexpr unsigned kMinusInf = 0xfc00fc00u;
+    static constexpr unsigned kMinusInf = 0xfc00fc00u, kNaN = 0x7fff7fffu;
 };
 
 // The largest of 16 bytes' elements and `top`, by words

@@ -52,3 +52,57 @@ def test_the_gradients_of_a_matrix_of_nearly_2_to_31_rows(cuda_lib):
     G[M - 3], G[M - 1] = 11.0, 13.0
     assert ops.sddmm(rp, ci, G, B).tolist() == [77.0, 11.0, 91.0]
     assert torch.ops.csrspmm_b200.spmm_transposed(rp, ci, va, G, Kd, 1.0).flatten().tolist() == [33.0, 0.0, 0.0, 0.0, 87.0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("T,V", [(2, 6001), (2000, 6001), (12000, 3001), (3000, 30011), (8, 60_000), (300, 150_003), (4, 300_003)])
+def test_distill_waits_that_run_out_leave_nan_and_nothing_unwritten(cuda_lib, monkeypatch, T, V, dtype):
+    """Without a single attempt for a copy every row is given up: NaN in the loss and in every element of the gradient, but for rows without a
+    teacher, which have nothing to wait for.  The context stays usable, and the next call is right."""
+    lens = torch.full((T,), 5)
+    lens[1::7] = 0
+    rp, ci, va = teacher(T, V, lens, 6)
+    x = torch.randn(T, V, device="cuda", generator=_gen(V)).to(dtype)
+    taught = (lens > 0).cuda()
+    good = ops.distill_loss_grad(x, rp, ci, va)
+    monkeypatch.setenv("CSRSPMM_TEST_WAIT_LIMIT", "0")
+    leaf = x.clone().requires_grad_(True)
+    alone = ops.distill_loss(leaf, rp, ci, va)
+    alone.sum().backward()
+    out = torch.full((T, V), 7.0, device="cuda", dtype=dtype)  # memory that the gradient may get, with something in it
+    del out
+    loss, dx = ops.distill_loss_grad(x, rp, ci, va)
+    torch.cuda.synchronize()
+    for l, d in ((loss, dx), (alone.detach(), leaf.grad)):
+        assert l[taught].isnan().all() and (l[~taught] == 0).all()
+        assert d[taught].isnan().all() and (d[~taught] == 0).all()
+    monkeypatch.delenv("CSRSPMM_TEST_WAIT_LIMIT")
+    again = ops.distill_loss_grad(x, rp, ci, va)
+    assert torch.equal(again[0], good[0]) and torch.equal(again[1], good[1]) and good[1].isfinite().all()
+
+
+@pytest.mark.parametrize("T,V,n", [(3000, 30_011, 20_000), (12_000, 3001, 6000), (80, 150_003, 40_000)])
+def test_distill_of_one_long_row_with_a_column_named_twice_among_short_ones(cuda_lib, T, V, n):
+    """The rows after it, of the same block and of the others of its cluster, wait for a walk over its entries."""
+    lens = torch.full((T,), 3)
+    at = [0, T // 2, T - 1]
+    lens[at] = n
+    order = torch.randint(0, V, (int(lens.sum()),), generator=torch.Generator().manual_seed(7))
+    rp = torch.zeros(T + 1, dtype=torch.int32)
+    rp[1:] = lens.cumsum(0)
+    va = torch.randn(order.numel(), generator=torch.Generator().manual_seed(8)).cuda()
+    rp, ci = rp.cuda(), order.int().cuda()
+    x = torch.randn(T, V, device="cuda", generator=_gen(V)).bfloat16()
+    loss, dx = ops.distill_loss_grad(x, rp, ci, va)
+    alone = ops.distill_loss(x, rp, ci, va)
+    assert loss.isfinite().all() and dx.isfinite().all() and alone.isfinite().all()
+    assert torch.allclose(alone, loss, rtol=1e-5, atol=1e-5)
+    # the rows about the long ones, on their own, are right and the same
+    some = torch.tensor(sorted({max(0, min(T - 1, r + d)) for r in at for d in (-1, 0, 1, 2)}), device="cuda")
+    part_rp = torch.zeros(some.numel() + 1, dtype=torch.int32, device="cuda")
+    part_rp[1:] = (rp[some + 1] - rp[some]).cumsum(0)
+    take = torch.cat([torch.arange(int(rp[r]), int(rp[r + 1]), device="cuda") for r in some.tolist()])
+    part = x[some], part_rp, ci[take].contiguous(), va[take].contiguous()
+    check_distill(*part)
+    want = ops.distill_loss_grad(*part)
+    assert torch.allclose(loss[some], want[0], rtol=1e-4, atol=1e-4) and torch.allclose(dx[some].float(), want[1].float(), rtol=2.0 ** -7, atol=1e-6)
