@@ -89,6 +89,9 @@ constexpr int kDynamicSmem = 216 * 1024;  // of a CTA, beside RingShared
 
 // The ring kernel's manager walks a row's entries with one warp; where rows have more than this many, all warps of the long kernel do.
 constexpr int kMostEntries = 2048;
+// And where one row may hold so many that its manager's walks over them (eight, each up to 25 cycles an entry) come near the limit of the waits for
+// it, 2^28 attempts of 20 cycles and more.
+constexpr long long kMostWalked = 1LL << 24;
 
 template <class T, int WORKERS, bool GRADIENT>
 cudaError_t launch_ring(const csrspmm_b200_distill_args* a, DistillParams p, int ctas_per_sm, cudaStream_t st)
@@ -96,7 +99,7 @@ cudaError_t launch_ring(const csrspmm_b200_distill_args* a, DistillParams p, int
     constexpr auto kernel = distill_ring_kernel<T, WORKERS, GRADIENT>;
     const int parts = 1 << p.log_parts;
     // A few waves of clusters, so that the SMs end together, of two to four rows each where there are as many.
-    p.rows = (int)std::clamp<long long>(((long long)a->T * parts) / ((long long)kSms * ctas_per_sm * 3), 1, WORKERS <= 128 ? 4 : 2);
+    p.rows = (int)std::clamp<long long>(((long long)a->T * parts) / ((long long)kSms * ctas_per_sm * 3), 1, WORKERS <= 128 ? kMostRows : 2);
     p.slots = WORKERS <= 128 ? std::min(p.rows, 2) : 1;
     const size_t smem = (size_t)p.ring_offset + (size_t)p.slots * p.slot_bytes;
     const cudaError_t e = allow_dynamic_smem<kernel>(smem);
@@ -121,7 +124,7 @@ cudaError_t launch_loss(const csrspmm_b200_distill_args* a, DistillParams p, cud
         });
     }
     const long long slot = (long long)p.per * size, before = GRADIENT ? ((long long)p.per / 32 + 1 + 31) / 32 * 128 : 0;
-    if (before + slot > kDynamicSmem || a->nnz / std::max(a->T, 1) > kMostEntries)
+    if (before + slot > kDynamicSmem || a->nnz / std::max(a->T, 1) > kMostEntries || a->nnz > kMostWalked)
         return for_type(a->logit_type, [&](auto zero) {
             return launch_clusters(distill_long_kernel<decltype(zero), GRADIENT>, grid, (unsigned)parts, kLongThreads, 0, st, p);
         });

@@ -102,8 +102,8 @@ struct Exponent {
     __device__ __forceinline__ float of_max(float other) const
     {
         const Exponent o(other, c);
-        if (!far && !o.far) return __fsub_rn(o.mc, mc);
-        return (other - m) * c + (excess() - o.excess());
+        const float apart = (other - m) * c + (excess() - o.excess());  // without a branch: lanes that hold nothing are far
+        return far || o.far ? apart : __fsub_rn(o.mc, mc);
     }
 };
 
@@ -342,23 +342,80 @@ __device__ __forceinline__ void store_vector(T* to, const uint4& v, bool aligned
     }
 }
 
-// The columns of the entries again, over what was written there: their p taken off.  A column that is named more than once is written by its first
-// entry, with all its p in stored order; `repeats`: there may be some.
+// What becomes of the columns of a row's entries where some may be named more than once: each is written with all its p.
+template <class T>
+struct NamedColumns {
+    float* sums;  // `span` floats of a warp's own
+    int span, part, parts;  // this warp's place among those that share the work
+    int c0, c1, V;          // columns that are written
+    Teacher t;
+    int log_probs;
+    float inv_t, c, m;       // of the exponentials
+    float scale, taken;      // dx = scale 2^y - taken * sum p
+    const T* x;
+    T* out;
+};
+
+// One warp's part: it walks over the entries once for every `span` columns and adds up their p in a fixed order, in time that grows with the entries
+// where comparing them with one another takes their square.
+template <class T, int U>  // U columns a lane on their way at once
+__device__ __forceinline__ void write_named_columns(NamedColumns<T> a)
+{
+    const int lane = threadIdx.x & 31;
+    const Exponent y(a.m, a.c);
+    for (long long base = a.c0 + (long long)a.part * a.span; base < a.c1; base += (long long)a.parts * a.span) {
+        const int from = (int)base, width = min(a.span, a.c1 - from);
+        for (int k = lane; k < width; k += 32) a.sums[k] = -1.0f;  // named by none
+        __syncwarp();
+        for (long long j0 = lane; j0 - lane < a.t.count; j0 += 32 * U) {
+            int at[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) at[u] = j0 + u * 32 < a.t.count ? min(max(__ldg(a.t.cols + j0 + u * 32), 0), a.V - 1) - from : -1;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool mine = at[u] >= 0 && at[u] < width;
+                if (!__any_sync(kAllLanes, mine)) continue;
+                float p = 0.0f;
+                if (mine) {
+                    const float v = __ldg(a.t.v + j0 + u * 32);
+                    p = a.log_probs ? expf(v) : v > -CUDART_INF_F ? expf((v - a.t.top) * a.inv_t) / a.t.sum : v != v ? v : 0.0f;
+                }
+                const unsigned same = __match_any_sync(kAllLanes, mine ? at[u] : -1 - lane);
+                if (__any_sync(kAllLanes, (same & (same - 1)) != 0)) {  // lanes of one column: each adds what follows it, by steps that double
+                    const unsigned above = same & ~((2u << lane) - 1u);
+                    int next = above != 0 ? __ffs(above) - 1 : -1;
+#pragma unroll
+                    for (int d = 0; d < 5; ++d) {
+                        const float v = __shfl_sync(kAllLanes, p, next & 31);
+                        const int n = __shfl_sync(kAllLanes, next, next & 31);
+                        if (next >= 0) p += v, next = n;
+                    }
+                }
+                if (mine && __ffs(same) - 1 == lane) a.sums[at[u]] = a.sums[at[u]] < 0.0f ? p : a.sums[at[u]] + p;
+                __syncwarp();
+            }
+        }
+        for (int k = lane; k < width; k += 32)
+            if (!(a.sums[k] < 0.0f)) a.out[from + k] = from_f32<T>(a.scale * exp2_approx(y.of(to_f32(a.x[from + k]))) - a.taken * a.sums[k]);
+        __syncwarp();
+    }
+}
+
+// The columns of the entries again, over what was written there: their p taken off.  `repeats`: a column may be named more than once; `sums`: `span`
+// floats for each warp.
 template <class T, int THREADS>
 __device__ __forceinline__ void write_entries(const DistillParams& p, const Entries<T, THREADS>& entries, const Teacher& t, const Exponent& y, float scale,
-                                              float weight, T* out, int c0, int c1, bool repeats)
+                                              float weight, T* out, int c0, int c1, bool repeats, float* sums, int span)
 {
-    entries.each([&](int i, const Entry& e) {
-        if (e.col < c0 || e.col >= c1) return;
-        float share = t.share(p, e.v);
-        if (repeats) {
-            for (int j = 0; j < i; ++j)
-                if (t.column(p, j) == e.col) return;
-            for (int j = i + 1; j < t.count; ++j)
-                if (t.column(p, j) == e.col) share += t.share(p, __ldg(t.v + j));
-        }
-        out[e.col] = from_f32<T>(scale * exp2_approx(y.of(e.x)) - weight * p.temperature * share);
-    });
+    if (repeats) {
+        const int warp = threadIdx.x >> 5;
+        write_named_columns<T, 4>({sums + warp * span, span, warp, THREADS / 32, c0, c1, p.V, t, p.log_probs, p.inv_t, y.c, y.m, scale,
+                                   weight * p.temperature, entries.row, out});
+    } else {
+        entries.each([&](int, const Entry& e) {
+            if (e.col >= c0 && e.col < c1) out[e.col] = from_f32<T>(scale * exp2_approx(y.of(e.x)) - weight * p.temperature * t.share(p, e.v));
+        });
+    }
 }
 
 // dx from the statistics that the loss left.  Grid: T rows of 2^log_parts CTAs.  A part has at most THREADS * NV vectors, all of which are
@@ -368,7 +425,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_gradient_kern
 {
     constexpr int N = Part<T>::N;
     constexpr int kNamedWords = THREADS * NV * N / 32 + 2;  // the part's vectors, and what is before and behind them
-    __shared__ unsigned named[kNamedWords];                 // a bit for each column of the part
+    constexpr int kSpan = 128;                              // for a warp's sums: at most 16 walks over the entries
+    __shared__ union {
+        unsigned named[kNamedWords];  // a bit for each column of the part
+        float sums[THREADS / 32 * kSpan];
+    } sh;
     wait_for_previous_grid();
     const Place at(p);
     const T* x = static_cast<const T*>(p.x) + (long long)at.row * p.ldx;
@@ -390,7 +451,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_gradient_kern
         return;
     }
     const Entries<T, THREADS> entries(p, t, x);
-    for (int i = threadIdx.x; i < kNamedWords; i += THREADS) named[i] = 0;
+    for (int i = threadIdx.x; i < kNamedWords; i += THREADS) sh.named[i] = 0;
     const float c = p.inv_t * CUDART_L2E_F;
     const Exponent y(stats.x, c);
     const float weight = __ldg(p.weight + at.row * p.weight_stride);
@@ -415,11 +476,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_gradient_kern
     if (named_here) {
         entries.each([&](int, const Entry& e) {
             const int k = e.col - at.c0;
-            if (k >= 0 && k < at.c1 - at.c0) repeats |= (atomicOr(&named[k >> 5], 1u << (k & 31)) >> (k & 31)) & 1u;
+            if (k >= 0 && k < at.c1 - at.c0) repeats |= (atomicOr(&sh.named[k >> 5], 1u << (k & 31)) >> (k & 31)) & 1u;
         });
     }
     repeats = __syncthreads_or(repeats);  // and what was written above comes before what is written below
-    if (named_here) write_entries<T, THREADS>(p, entries, t, y, scale, weight, out, at.c0, at.c1, repeats);
+    if (named_here || repeats) write_entries<T, THREADS>(p, entries, t, y, scale, weight, out, at.c0, at.c1, repeats, sh.sums, kSpan);
 }
 
 // Short rows: a warp each, which holds its row in registers, up to NV vectors a lane.  (Under the ring's two warps of a CTA a row of 1500 bf16
@@ -429,7 +490,12 @@ constexpr int kShortThreads = 256;
 template <class T, int NV, bool GRADIENT>
 __global__ void __launch_bounds__(kShortThreads) distill_short_kernel(DistillParams p)
 {
-    constexpr int N = Part<T>::N;
+    constexpr int N = Part<T>::N, kSpan = 256;
+    static_assert(kSpan * 32 >= 32 * NV * N, "a bit for each column of a row");
+    __shared__ union {
+        unsigned named[kSpan];
+        float sums[kSpan];
+    } of_warp[GRADIENT ? kShortThreads / 32 : 1];
     wait_for_previous_grid();
     const int lane = threadIdx.x & 31;
     const int row = (int)(blockIdx.x * (kShortThreads / 32) + (threadIdx.x >> 5));
@@ -521,26 +587,24 @@ __global__ void __launch_bounds__(kShortThreads) distill_short_kernel(DistillPar
         else write(std::false_type());
         if (edge_col >= 0) out[edge_col] = from_f32<T>(zero ? 0.0f : scale * exp2_approx(y.of(edge)));
         if (zero) return;
-        bool repeats = false;  // ascending columns name none twice, nor do 32 that all differ
+        bool repeats = false;
+        auto& sh = of_warp[threadIdx.x >> 5];
         if (t.count <= 32) {
             const unsigned same = __match_any_sync(kAllLanes, lane < t.count ? first.col : -1 - lane);
-            repeats = __any_sync(kAllLanes, (same & (same - 1)) != 0);
+            repeats = (same & (same - 1)) != 0;
         } else {
-            for (int j = lane; j + 1 < t.count; j += 32) repeats |= t.column(p, j) >= t.column(p, j + 1);
-            repeats = __any_sync(kAllLanes, repeats);
+            for (int k = lane; k * 32 < p.V; k += 32) sh.named[k] = 0;
+            __syncwarp();
+            each([&](int, const Entry& e) { repeats |= (atomicOr(&sh.named[e.col >> 5], 1u << (e.col & 31)) >> (e.col & 31)) & 1u; });
         }
+        repeats = __any_sync(kAllLanes, repeats);
         __syncwarp();  // what was written above comes before what is written below
         const auto share_of = [&](float v) { return p.log_probs ? expf(v) : expf(over_of(v)) / t.sum; };
-        each([&](int j, const Entry& e) {
-            float taken = share_of(e.v);
-            if (repeats) {  // a column named more than once is written by its first entry, with all its p in stored order
-                for (int q = 0; q < j; ++q)
-                    if (t.column(p, q) == e.col) return;
-                for (int q = j + 1; q < t.count; ++q)
-                    if (t.column(p, q) == e.col) taken += share_of(__ldg(t.v + q));
-            }
-            out[e.col] = from_f32<T>(scale * exp2_approx(y.of(e.x)) - weight * p.temperature * taken);
-        });
+        if (repeats) {
+            write_named_columns<T, 2>({sh.sums, kSpan, 0, 1, 0, p.V, p.V, t, p.log_probs, p.inv_t, c, y.m, scale, weight * p.temperature, x, out});
+        } else {
+            each([&](int, const Entry& e) { out[e.col] = from_f32<T>(scale * exp2_approx(y.of(e.x)) - weight * p.temperature * share_of(e.v)); });
+        }
     }
 }
 
@@ -553,12 +617,13 @@ __global__ void __launch_bounds__(kShortThreads) distill_short_kernel(DistillPar
 
 constexpr int kListed = 256;  // entries of a row that are kept in shared memory; rows with more read them where they need them
 constexpr int kMostSlots = 2;
+constexpr int kMostRows = 4;  // of a CTA or cluster
 // How much longer than a copy takes may be waited for what a manager does first, who may still walk over the entries of the row before.
 constexpr unsigned kWalkFactor = 64;
 constexpr unsigned kToldLimit = kWalkFactor * kWaitSpinLimit;
 
-// From so many entries on the copy of a later row is asked for before the walk that writes the entries' columns, which then reads its logits from
-// memory: the workers wait for a copy, not for the walk.
+// From so many entries on the walk that writes the entries' columns comes after all rows, with the logits from memory, as it does where columns are
+// named twice in more than a list: the workers wait for a copy, not for the walk.
 constexpr int kLongWalk = 2048;
 
 struct RingRow {  // what the workers need to write a part of dx
@@ -569,6 +634,11 @@ struct RingRow {  // what the workers need to write a part of dx
 
 struct RingBlock {  // what a part hands to the others: its maximum and sum, and over its entries sum e (v / t - (z - max z)), sum e
     float m, s, cross, share;
+};
+
+struct RingLate {  // a row whose entries' columns are written after all others
+    int row, kind;  // kind 0: nothing to write, 1: every column is named once, 2: some more than once
+    float m, scale, taken, top, sum;
 };
 
 template <int WORKERS>
@@ -583,6 +653,7 @@ struct RingShared {
     alignas(8) unsigned long long told[2];           // the blocks of a row have
     int dead;                                        // something did not within the limit: from there on the loss and gradient of every row are NaN
     int joined;                                      // rows whose sums the manager has taken
+    RingLate late[kMostRows];
 };
 
 // Barriers of the CTA by number, for `threads` threads: arriving does not wait.
@@ -776,17 +847,16 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
         fetch_entries(1, offsets[1], offsets[2]);
         float next_edge = fetch_edge(0), next_weight = weight_of(0);
         Teacher next = teach(0, offsets[0], offsets[1]);
-        int slot = 0;
+        int slot = 0, late = 0;
         unsigned phase = 0;
         for (int i = 0; i < rows; ++i) {
             const Place at(p, first_row + i);
             const T* x = all_x + (long long)at.row * p.ldx;
             const Part<T> part(x, at.c0, at.c1);
             const T* const here = reinterpret_cast<const T*>(ring + slot * p.slot_bytes);
-            bool held = true;                            // the slot is still this row's
             const auto element = [&](int col) {  // of this part
                 const int k = col - part.first;
-                return to_f32(held && k >= 0 && k < part.vectors * N ? here[k] : x[col]);
+                return to_f32(k >= 0 && k < part.vectors * N ? here[k] : x[col]);
             };
             const Teacher t = next;
             const bool listed = t.count <= kListed, counts = t.top != -CUDART_INF_F;
@@ -893,50 +963,52 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
                 };
                 const auto inside = [&](int col) { return !zero && col >= at.c0 && col < at.c1; };
                 bool repeats = false;
+                unsigned again = 0, bit = 1;  // which of this lane's listed entries name a column that one before has marked
                 if (!zero) {
                     for (int j = lane; j < t.count; j += 32) {
                         const int col = column(j), k = col - at.c0;
-                        if (inside(col)) repeats |= (atomicOr(&named[k >> 5], 1u << (k & 31)) >> (k & 31)) & 1u;
+                        if (inside(col) && ((atomicOr(&named[k >> 5], 1u << (k & 31)) >> (k & 31)) & 1u)) again |= bit;
+                        bit = __funnelshift_l(bit, bit, 1);  // beyond a list's eight it only counts that there are some
                     }
-                    repeats = __any_sync(kAllLanes, repeats);
+                    repeats = __any_sync(kAllLanes, again != 0);
                     for (int j = lane; j < t.count; j += 32)
                         if (inside(column(j))) named[(column(j) - at.c0) >> 5] = 0;
                 }
-                const bool ready = listed && !repeats;  // what becomes of the entries' columns is known before the workers are done
-                const auto next_copy = [&] {
-                    if (arrived && i + p.slots < rows) {  // everybody has read the slot
-                        if (lane == 0) fence_proxy_async_smem();
-                        issue(i + p.slots, slot);
+                if (listed) {  // what becomes of a list's columns is known before the workers are done
+                    unsigned done = 0;
+                    // columns that are named again, one at a time, with all their p, whichever of their entries marked them first
+                    while (repeats) {
+                        const unsigned left = __ballot_sync(kAllLanes, again != 0);
+                        if (left == 0) break;
+                        const int whose = __ffs(left) - 1, col = column(__shfl_sync(kAllLanes, __ffs(again) - 1, whose) * 32 + whose);
+                        float taken = 0.0f;
+                        for (int j = lane; j < t.count; j += 32)
+                            if (column(j) == col) taken += share_of(j);
+                        const float g = gradient(col, warp_sum(taken));
+                        for (int j = lane; j < t.count; j += 32)
+                            if (column(j) == col) sh.v[i % 3][j] = g, done |= 1u << (j / 32);
+                        again &= ~done;
                     }
-                };
-                if (ready) {
-                    for (int j = lane; j < t.count; j += 32)
-                        if (inside(column(j))) sh.v[i % 3][j] = gradient(column(j), share_of(j));
+                    for (int j = lane; j < t.count; j += 32, done >>= 1)
+                        if (inside(column(j)) && !(done & 1u)) sh.v[i % 3][j] = gradient(column(j), share_of(j));
                 }
                 if (i + 1 < rows) next = teach(i + 1, offsets[1], offsets[2]);
                 barrier_sync(kWritten + slot, ALL);  // what the workers wrote comes before what is written here
-                if (!ready) {
+                if (!listed) {
                     if (repeats || t.count > kLongWalk) {
-                        held = false;
-                        next_copy();
+                        if (lane == 0) sh.late[late] = {at.row, zero ? 0 : repeats ? 2 : 1, y.m, scale, weight * p.temperature, t.top, t.sum};
+                        ++late;
+                    } else {
+                        for (int j = lane; j < t.count; j += 32)
+                            if (inside(column(j))) out[column(j)] = from_f32<T>(gradient(column(j), share_of(j)));
+                        __syncwarp();
                     }
-                    for (int j = lane; j < t.count; j += 32) {
-                        const int col = column(j);
-                        if (!inside(col)) continue;
-                        float taken = share_of(j);
-                        if (repeats) {  // a column named more than once is written by its first entry, with all its p in stored order
-                            bool first = true;
-                            for (int q = 0; q < j && first; ++q) first = column(q) != col;
-                            if (!first) continue;
-                            for (int q = j + 1; q < t.count; ++q)
-                                if (column(q) == col) taken += share_of(q);
-                        }
-                        out[col] = from_f32<T>(gradient(col, taken));
-                    }
-                    __syncwarp();
                 }
-                if (held) next_copy();
-                if (ready) {
+                if (arrived && i + p.slots < rows) {  // everybody has read the slot
+                    if (lane == 0) fence_proxy_async_smem();
+                    issue(i + p.slots, slot);
+                }
+                if (listed) {
                     for (int j = lane; j < t.count; j += 32)
                         if (inside(column(j))) out[column(j)] = from_f32<T>(sh.v[i % 3][j]);
                 }
@@ -949,6 +1021,28 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
             if (++slot == p.slots) slot = 0, phase ^= 1;
         }
         async_wait<0>();
+        if constexpr (GRADIENT) {
+            __syncwarp();
+            for (int k = 0; k < late; ++k) {  // nobody waits for these
+                const RingLate l = sh.late[k];
+                const Place at(p, l.row);
+                Teacher t = teacher_of(p, __ldg(p.row_ptr + l.row), __ldg(p.row_ptr + l.row + 1));
+                t.top = l.top;
+                t.sum = p.log_probs ? 1.0f : l.sum;
+                const T* const x = all_x + (long long)l.row * p.ldx;
+                T* const out = static_cast<T*>(p.dx) + (long long)l.row * p.ldd;
+                if (l.kind == 2) {  // the bits are as many as a 32nd of the columns: 32 walks over the entries
+                    write_named_columns<T, 4>({reinterpret_cast<float*>(named), p.ring_offset / 4, 0, 1, at.c0, at.c1, p.V, t, p.log_probs, p.inv_t, c, l.m,
+                                               l.scale, l.taken, x, out});
+                } else if (l.kind == 1) {
+                    const Exponent y(l.m, c);
+                    for (int j = lane; j < t.count; j += 32) {
+                        const int col = t.column(p, j);
+                        if (col >= at.c0 && col < at.c1) out[col] = from_f32<T>(l.scale * exp2_approx(y.of(to_f32(x[col]))) - l.taken * t.share(p, __ldg(t.v + j)));
+                    }
+                }
+            }
+        }
         if (*dead != 0 && lane == 0) {  // no copy may arrive after the CTA has gone
             for (int i = max(issued - p.slots, 0); i < issued; ++i) mbar_wait_bounded(smem_u32(&sh.full[i % p.slots]), (unsigned)(i / p.slots) & 1u);
         }
@@ -964,7 +1058,12 @@ template <class T, bool GRADIENT>
 __global__ void __launch_bounds__(kLongThreads, 2) distill_long_kernel(DistillParams p)
 {
     constexpr int N = Part<T>::N, THREADS = kLongThreads;
+    constexpr int kSpan = 512;
     __shared__ Room<THREADS> room;
+    __shared__ union {
+        unsigned named[THREADS / 32 * kSpan];
+        float sums[THREADS / 32 * kSpan];
+    } sh;
     wait_for_previous_grid();
     const Place at(p);
     const T* x = static_cast<const T*>(p.x) + (long long)at.row * p.ldx;
@@ -1040,11 +1139,24 @@ __global__ void __launch_bounds__(kLongThreads, 2) distill_long_kernel(DistillPa
                     if (k + u * THREADS < part.vectors) store_vector(to + (long long)(k + u * THREADS) * N, Words<T>::map(v[u], value), aligned);
             }
             if (part.edge >= 0) out[part.edge] = from_f32<T>(scale * exp2_approx(y.of(edge)));
-            // ascending columns name none twice
+            // ascending columns name none twice; of others the part's are marked, a bit each, as many at once as there is room for
             bool repeats = false;
             for (int i = threadIdx.x; i + 1 < t.count; i += THREADS) repeats |= t.column(p, i) >= t.column(p, i + 1);
-            repeats = __syncthreads_or(repeats);
-            write_entries<T, THREADS>(p, entries, t, y, scale, weight, out, at.c0, at.c1, repeats);
+            if (__syncthreads_or(repeats)) {
+                constexpr int kMarked = THREADS * kSpan;
+                repeats = false;
+                for (long long base = at.c0; base < at.c1; base += kMarked) {
+                    for (int i = threadIdx.x; i < kMarked / 32; i += THREADS) sh.named[i] = 0;
+                    __syncthreads();
+                    for (int i = threadIdx.x; i < t.count; i += THREADS) {
+                        const long long k = t.column(p, i) - base;
+                        if (k >= 0 && k < min((long long)kMarked, at.c1 - base)) repeats |= (atomicOr(&sh.named[k >> 5], 1u << (k & 31)) >> (k & 31)) & 1u;
+                    }
+                    repeats = __syncthreads_or(repeats);
+                    if (repeats) break;
+                }
+            }
+            write_entries<T, THREADS>(p, entries, t, y, scale, weight, out, at.c0, at.c1, repeats, sh.sums, kSpan);
         }
     }
     leave_row(p.log_parts);

@@ -81,13 +81,19 @@ def test_distill_waits_that_run_out_leave_nan_and_nothing_unwritten(cuda_lib, mo
     assert torch.equal(again[0], good[0]) and torch.equal(again[1], good[1]) and good[1].isfinite().all()
 
 
-@pytest.mark.parametrize("T,V,n", [(3000, 30_011, 20_000), (12_000, 3001, 6000), (80, 150_003, 40_000)])
-def test_distill_of_one_long_row_with_a_column_named_twice_among_short_ones(cuda_lib, T, V, n):
-    """The rows after it, of the same block and of the others of its cluster, wait for a walk over its entries."""
+@pytest.mark.parametrize("twice", [False, True])
+@pytest.mark.parametrize("T,V,n", [(3000, 30_011, 20_000), (3000, 30_011, 1000), (12_000, 3001, 3000), (12_000, 6001, 400), (80, 150_003, 40_000)])
+def test_distill_of_one_long_row_among_short_ones(cuda_lib, T, V, n, twice):
+    """The rows after it, of the same block and of the others of its cluster, wait for a walk over its entries, which may name a column twice."""
     lens = torch.full((T,), 3)
     at = [0, T // 2, T - 1]
     lens[at] = n
-    order = torch.randint(0, V, (int(lens.sum()),), generator=torch.Generator().manual_seed(7))
+    gen = torch.Generator().manual_seed(7)
+    order = torch.randint(0, V, (int(lens.sum()),), generator=gen)
+    if not twice:
+        ends = lens.cumsum(0)
+        for r in at:
+            order[ends[r] - n : ends[r]] = torch.randperm(V, generator=gen)[:n]
     rp = torch.zeros(T + 1, dtype=torch.int32)
     rp[1:] = lens.cumsum(0)
     va = torch.randn(order.numel(), generator=torch.Generator().manual_seed(8)).cuda()
@@ -106,3 +112,28 @@ def test_distill_of_one_long_row_with_a_column_named_twice_among_short_ones(cuda
     check_distill(*part)
     want = ops.distill_loss_grad(*part)
     assert torch.allclose(loss[some], want[0], rtol=1e-4, atol=1e-4) and torch.allclose(dx[some].float(), want[1].float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("V,k", [(300, 33), (1000, 700), (1500, 256), (9001, 300), (60_000, 2000), (9001, 5000), (600_000, 3000), (3_000_000, 2500)])
+@pytest.mark.parametrize("kind", ["unsorted", "twice", "same", "padded"])
+def test_distill_of_many_entries_in_any_order(cuda_lib, V, k, kind, dtype):
+    T = 3
+    rp, ci, va = teacher(T, V, [min(k, V)] * T, 9)
+    ci = ci.view(T, -1)
+    n = ci.shape[1]
+    if kind == "twice":
+        ci[0, n // 2] = ci[0, 3]
+        ci[1] = torch.randint(0, V, (n,), device="cuda", generator=_gen(10)).int()
+        ci[2, : n // 2] = ci[2, n - n // 2 :]
+    elif kind == "same":
+        ci[0] = V - 1
+        ci[1] = torch.where(torch.arange(n, device="cuda") % 3 == 0, V // 2, ci[1])
+        ci[2] = torch.arange(n, device="cuda").int() // 32 * 7 % V
+    elif kind == "padded":  # lists of a length that is the same for all, filled up with a column that weighs nothing
+        ci[:, n // 3 :] = 0
+        va.view(T, -1)[:, n // 3 :] = -float("inf")
+    x = torch.randn(T, V, device="cuda", generator=_gen(V)).to(dtype)
+    check_distill(x, rp, ci.flatten().contiguous(), va)
+    a, b = ops.distill_loss_grad(x, rp, ci.flatten(), va), ops.distill_loss_grad(x, rp, ci.flatten(), va)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
