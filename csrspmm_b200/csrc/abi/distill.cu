@@ -87,8 +87,11 @@ constexpr int kPartBytes = 100 * 1024;    // of a part, as far as clusters go: t
 constexpr int kFewBytes = 32768;          // up to here four warps do as well as eight, and six CTAs fit an SM (9000 bf16 columns: 192 -> 143 us for 16384 rows)
 constexpr int kDynamicSmem = 216 * 1024;  // of a CTA, beside RingShared
 
-// The ring kernel's manager walks a row's entries with one warp; where rows have more than this many, all warps of the long kernel do.
-constexpr int kMostEntries = 2048;
+// The ring kernel's manager is one warp, and holds up to kListed entries of a row in shared memory; where rows have more, all warps of the long kernel
+// walk over them.  Loss and gradient with 256, 384 and 1024 entries a row of bf16 logits, by the ring and by the long kernel: 16384 rows of 3000 columns 261, 531, 1285
+// and 304, 328, 471 us, of 9000 282, 747, 1947 and 355, 374, 545, 4096 of 30000 124, 316, 752 and 149, 152, 202, 2048 of 131072 270, 640, 1481
+// and 355, 360, 443, 64 of 131072 15, 24, 51 and 19, 20, 25.  With 32 the ring takes 0.4 to 0.65 of the other's time, but for 128 of 600000 (115 and 92).
+constexpr int kMostEntries = kListed;
 // And where one row may hold so many that its manager's walks over them (eight, each up to 25 cycles an entry) come near the limit of the waits for
 // it, 2^28 attempts of 20 cycles and more.
 constexpr long long kMostWalked = 1LL << 24;

@@ -181,6 +181,16 @@ def test_nothing_is_compiled_that_no_call_launches(fake):
     assert every and sorted(every - _names(fake.fake_launched)) == []
 
 
+def test_rows_of_more_entries_than_a_list_holds_take_the_kernel_in_which_all_warps_walk_over_them(fake):
+    for T, V in ((1000, 100_000), (20_000, 6000)):
+        for per_row, ring in ((64, True), (256, True), (257, False), (2048, False)):
+            a = _distill(T=T, V=V, ld=V, nnz=T * per_row)
+            fake.fake_reset(0)
+            assert fake.csrspmm_b200_distill(C.byref(a), P, P, None) == 0 and fake.csrspmm_b200_distill_grad(C.byref(a), P, 1, P, P, V, None) == 0
+            names = _names(fake.fake_launched)
+            assert len(names) == 2 and all(("distill_ring_kernel" if ring else "distill_long_kernel") in n for n in names)
+
+
 def test_a_failed_launch_is_reported(fake):
     for run in (lambda: fake.csrspmm_b200_route(C.byref(_route()), P, P, P, None),
                 lambda: fake.csrspmm_b200_route_backward(C.byref(_route()), P, P, P, 1, P, 64, None),
