@@ -105,7 +105,24 @@ struct Exponent {
         const float apart = (other - m) * c + (excess() - o.excess());  // without a branch: lanes that hold nothing are far
         return far || o.far ? apart : __fsub_rn(o.mc, mc);
     }
+    // (x - m) / t for the loss, where x log2(e) / t may pass fp32 while x / t does not: a teacher's entry where the student holds the type's lowest
+    __device__ __forceinline__ float below(float x, float inv_t) const { return natural(of(x), x, inv_t); }
+    __device__ __forceinline__ float max_below(float other, float inv_t) const { return natural(of_max(other), other, inv_t); }
+    __device__ __forceinline__ float natural(float y, float x, float inv_t) const
+    {
+        return fabsf(y) <= -kLowest ? y * CUDART_LN2_F : x * inv_t - m * inv_t;
+    }
 };
+
+// The entries' sum of e (v / t - (z - max z)) is kept in this unit where e is relative to the largest: a few e of 1 times the type's lowest pass fp32
+// before they are divided by the sum of the e.  (With log_probs the e are the p themselves.)
+constexpr float kCrossUnit = 5.9604644775390625e-8f, kPerCrossUnit = 16777216.0f;  // 2^-24
+__device__ __forceinline__ float cross_unit(const DistillParams& p) { return p.log_probs ? 1.0f : kCrossUnit; }
+// A row's loss but for t^2; sum: sum e, mass: P, lse: the logarithm of the sum of exp(z - max z)
+__device__ __forceinline__ float divergence(const DistillParams& p, float cross, float sum, float mass, float lse)
+{
+    return p.log_probs ? cross + mass * lse : cross / sum * kPerCrossUnit - logf(sum) + lse;
+}
 
 // A maximum and the sum of 2^y relative to it; none: kLowest and 0.
 struct MaxSum {
@@ -281,13 +298,14 @@ __device__ __forceinline__ float finish_loss(const DistillParams& p, const Place
     constexpr int W = THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // with e = exp((v - top) / t): sum e, and sum e ((v - top) / t - (z - max z))
+    const float unit = cross_unit(p);
     float sum = 0.0f, cross = 0.0f;
     if (warp * 32 < t.count) {
         entries.each([&](int, const Entry& e) {
             const float over = p.log_probs ? e.v : (e.v - t.top) * p.inv_t;
             const float share = expf(over);
             sum += share;
-            if (share != 0.0f) cross += share * (over - y.of(e.x) * CUDART_LN2_F);
+            if (share != 0.0f) cross += share * ((over - y.below(e.x, p.inv_t)) * unit);
         });
         sum = warp_sum(sum);
         cross = warp_sum(cross);
@@ -303,7 +321,7 @@ __device__ __forceinline__ float finish_loss(const DistillParams& p, const Place
         cross = warp_sum(lane < W ? room.cross[lane] : 0.0f);
         if (lane == 0) {
             const float lse = logf(s), tt = p.temperature * p.temperature;
-            p.loss[at.row] = mass == 0.0f ? 0.0f : tt * (p.log_probs ? cross + mass * lse : cross / sum - logf(sum) + lse);
+            p.loss[at.row] = mass == 0.0f ? 0.0f : tt * divergence(p, cross, sum, mass, lse);
             if (p.stats != nullptr) p.stats[at.row] = make_float4(y.m, s, t.top, sum);
         }
     }
@@ -555,12 +573,13 @@ __global__ void __launch_bounds__(kShortThreads) distill_short_kernel(DistillPar
     }
     const bool counts = t.top != -CUDART_INF_F;  // some entry weighs something
     const auto over_of = [&](float v) { return p.log_probs ? v : (v - t.top) * p.inv_t; };
+    const float unit = cross_unit(p);
     float cross = 0.0f;
     if (counts) {
         each([&](int, const Entry& e) {
             const float over = over_of(e.v), share = expf(over);
             t.sum += share;
-            if (share != 0.0f) cross += share * (over - y.of(e.x) * CUDART_LN2_F);
+            if (share != 0.0f) cross += share * ((over - y.below(e.x, p.inv_t)) * unit);
         });
         t.sum = warp_sum(t.sum);
         cross = warp_sum(cross);
@@ -569,7 +588,7 @@ __global__ void __launch_bounds__(kShortThreads) distill_short_kernel(DistillPar
     const bool zero = mass == 0.0f;
     if (lane == 0) {
         const float lse = logf(s), tt = p.temperature * p.temperature;
-        p.loss[row] = zero ? 0.0f : tt * (p.log_probs ? cross + mass * lse : cross / t.sum - logf(t.sum) + lse);
+        p.loss[row] = zero ? 0.0f : tt * divergence(p, cross, t.sum, mass, lse);
         if (p.stats != nullptr) p.stats[row] = counts ? make_float4(y.m, s, t.top, t.sum) : make_float4(0.0f, 1.0f, -CUDART_INF_F, 1.0f);
     }
     if constexpr (GRADIENT) {
@@ -632,7 +651,7 @@ struct RingRow {  // what the workers need to write a part of dx
     void* to;
 };
 
-struct RingBlock {  // what a part hands to the others: its maximum and sum, and over its entries sum e (v / t - (z - max z)), sum e
+struct RingBlock {  // what a part hands to the others: its maximum and sum, and over its entries sum e (v / t - (z - max z)) in units, sum e
     float m, s, cross, share;
 };
 
@@ -816,6 +835,7 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
             return col >= 0 ? to_f32(x[col]) : -CUDART_INF_F;
         };
         const auto value_of = [&](const Teacher& t, int i, int j) { return t.count <= kListed ? sh.v[i % 3][j] : __ldg(t.v + j); };
+        const float unit = cross_unit(p);
         const auto over_of = [&](const Teacher& t, float v) { return p.log_probs ? v : (v - t.top) * p.inv_t; };
         const auto teach = [&](int i, int from, int to) {  // row i's shares: exp(over_of) / sum; top is -infinity where none weighs anything
             Teacher t = teacher_of(p, from, to);
@@ -885,7 +905,7 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
                     if (col >= at.c0 && col < at.c1) {
                         const float over = over_of(t, value_of(t, i, j)), e = expf(over);
                         share += e;
-                        if (e != 0.0f) cross += e * (over - y.of(element(col)) * CUDART_LN2_F);
+                        if (e != 0.0f) cross += e * ((over - y.below(element(col), p.inv_t)) * unit);
                     }
                 }
                 cross = warp_sum(cross);
@@ -901,7 +921,7 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
             const int whose = lane % kJoined;
             MaxSum mine = join_lanes<kJoined>(whose < W ? sh.part[slot][whose] : whose == W ? edges : MaxSum{kLowest, 0.0f}, c);
             if (!arrived) mine.s = CUDART_NAN_F;
-            if (share != 0.0f) cross -= Exponent(mine.m, c).of_max(top) * CUDART_LN2_F * share;
+            if (share != 0.0f) cross -= Exponent(mine.m, c).max_below(top, p.inv_t) * unit * share;
             if constexpr (!GRADIENT) {
                 if (arrived && i + p.slots < rows) {  // everybody has read the slot
                     if (lane == 0) fence_proxy_async_smem();
@@ -941,11 +961,11 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
             }
             if (rank == 0) {
                 float crosses = 0.0f;
-                if (lane < parts) crosses = block.cross - (block.share != 0.0f ? y.of_max(block.m) * CUDART_LN2_F * block.share : 0.0f);
+                if (lane < parts) crosses = block.cross - (block.share != 0.0f ? y.max_below(block.m, p.inv_t) * unit * block.share : 0.0f);
                 crosses = warp_sum(crosses);
                 if (lane == 0) {
                     const float lse = logf(all.s), tt = p.temperature * p.temperature;
-                    p.loss[at.row] = zero ? 0.0f : tt * (p.log_probs ? crosses + mass * lse : crosses / t.sum - logf(t.sum) + lse);
+                    p.loss[at.row] = zero ? 0.0f : tt * divergence(p, crosses, t.sum, mass, lse);
                     if (p.stats != nullptr)
                         p.stats[at.row] = counts ? make_float4(all.m, all.s, t.top, t.sum) : make_float4(0.0f, 1.0f, -CUDART_INF_F, 1.0f);
                 }

@@ -408,7 +408,7 @@ int csrspmm_b200_spmm_transposed(int32_t M, int32_t Kd, int32_t Nd, int64_t nnz,
  *     dlogits_j = weight * t * (P q_j - sum of the p_i with col_i = j)
  * A row without entries, or with none that weighs anything, has loss 0 and gradient 0 whatever its logits hold.  Entries may come in any
  * order; a column named twice counts with both.  A column outside [0, V) counts as the nearest one inside.
- * Logits are fp32, fp16 or bf16, computed with in fp32. */
+ * Logits are fp32, fp16 or bf16, computed with in fp32: a loss is finite as long as z and the loss itself are in fp32. */
 typedef struct csrspmm_b200_distill_args {
     uint32_t struct_size; /* sizeof(csrspmm_b200_distill_args), checked */
     int32_t T, V;

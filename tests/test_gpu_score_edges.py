@@ -137,3 +137,24 @@ def test_distill_of_many_entries_in_any_order(cuda_lib, V, k, kind, dtype):
     check_distill(x, rp, ci.flatten().contiguous(), va)
     a, b = ops.distill_loss_grad(x, rp, ci.flatten(), va), ops.distill_loss_grad(x, rp, ci.flatten(), va)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("t", [1.0, 1.2, 2.0])
+@pytest.mark.parametrize("log_probs", [False, True])
+@pytest.mark.parametrize("V", [300, 20000, 150_000, 600_000])
+def test_distill_from_a_teacher_who_wants_what_is_masked_by_the_lowest(cuda_lib, V, log_probs, t, dtype):
+    """The loss is as large as the mask, and finite: p * lowest."""
+    T, k = 4, 12
+    x = torch.randn(T, V, device="cuda", generator=_gen(V)).to(dtype)
+    rp, ci, _ = teacher(T, V, [k] * T, 4)
+    va = torch.full((T, k), -4.0, device="cuda")
+    hit = ci.long().view(T, k)
+    lowest = torch.finfo(dtype).min
+    x[0, hit[0, 3]] = lowest
+    x[1, hit[1, ::6]] = lowest  # two of equal weight: their sum before it is divided is beyond fp32
+    va[2, 7] = -2.0
+    x[2, hit[2, 7]] = lowest
+    x[3, hit[3, 1]] = -1e38
+    check_distill(x, rp, ci, va.flatten(), t, log_probs)
+    assert ops.distill_loss(x, rp, ci, va.flatten(), temperature=t, log_probs=log_probs).isfinite().all()
