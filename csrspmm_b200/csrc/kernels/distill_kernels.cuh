@@ -982,24 +982,31 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
                     return scale * exp2_approx(y.of(element(col))) - weight * p.temperature * taken;
                 };
                 const auto inside = [&](int col) { return !zero && col >= at.c0 && col < at.c1; };
-                bool repeats = false;
-                unsigned again = 0, bit = 1;  // which of this lane's listed entries name a column that one before has marked
-                if (!zero) {
-                    for (int j = lane; j < t.count; j += 32) {
-                        const int col = column(j), k = col - at.c0;
-                        if (inside(col) && ((atomicOr(&named[k >> 5], 1u << (k & 31)) >> (k & 31)) & 1u)) again |= bit;
-                        bit = __funnelshift_l(bit, bit, 1);  // beyond a list's eight it only counts that there are some
-                    }
-                    repeats = __any_sync(kAllLanes, again != 0);
+                // whether entry j's column is marked before
+                const auto marked = [&](int j) {
+                    const int col = column(j), k = col - at.c0;
+                    return inside(col) && ((atomicOr(&named[k >> 5], 1u << (k & 31)) >> (k & 31)) & 1u) != 0;
+                };
+                const auto unmark = [&] {
+                    __syncwarp();
                     for (int j = lane; j < t.count; j += 32)
                         if (inside(column(j))) named[(column(j) - at.c0) >> 5] = 0;
+                };
+                bool repeats = false;
+                if (!zero) {
+                    for (int j = lane; j < t.count; j += 32) repeats |= marked(j);
+                    repeats = __any_sync(kAllLanes, repeats);
+                    unmark();
                 }
-                if (listed) {  // what becomes of a list's columns is known before the workers are done
-                    unsigned done = 0;
-                    // columns that are named again, one at a time, with all their p, whichever of their entries marked them first
-                    while (repeats) {
-                        const unsigned left = __ballot_sync(kAllLanes, again != 0);
-                        if (left == 0) break;
+                if (listed && !repeats) {  // what becomes of a list's columns is known before the workers are done
+                    for (int j = lane; j < t.count; j += 32)
+                        if (inside(column(j))) sh.v[i % 3][j] = gradient(column(j), share_of(j));
+                } else if (listed) {  // columns that are named again, one at a time, with all their p, whichever of their entries marks them first
+                    __syncwarp();
+                    unsigned again = 0, done = 0;
+                    for (int j = lane; j < t.count; j += 32) again |= (unsigned)marked(j) << (j / 32);
+                    unmark();
+                    for (unsigned left; (left = __ballot_sync(kAllLanes, again != 0)) != 0; again &= ~done) {
                         const int whose = __ffs(left) - 1, col = column(__shfl_sync(kAllLanes, __ffs(again) - 1, whose) * 32 + whose);
                         float taken = 0.0f;
                         for (int j = lane; j < t.count; j += 32)
@@ -1007,10 +1014,9 @@ __global__ void __launch_bounds__(WORKERS + 32, WORKERS == 128 ? 6 : WORKERS == 
                         const float g = gradient(col, warp_sum(taken));
                         for (int j = lane; j < t.count; j += 32)
                             if (column(j) == col) sh.v[i % 3][j] = g, done |= 1u << (j / 32);
-                        again &= ~done;
                     }
-                    for (int j = lane; j < t.count; j += 32, done >>= 1)
-                        if (inside(column(j)) && !(done & 1u)) sh.v[i % 3][j] = gradient(column(j), share_of(j));
+                    for (int j = lane; j < t.count; j += 32)
+                        if (inside(column(j)) && !((done >> (j / 32)) & 1u)) sh.v[i % 3][j] = gradient(column(j), share_of(j));
                 }
                 if (i + 1 < rows) next = teach(i + 1, offsets[1], offsets[2]);
                 barrier_sync(kWritten + slot, ALL);  // what the workers wrote comes before what is written here
