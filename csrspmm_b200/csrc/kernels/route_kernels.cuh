@@ -92,11 +92,13 @@ __device__ __forceinline__ bool whole_vectors(const void* x, long long ld, int E
     return E % N == 0 && ld % N == 0 && (reinterpret_cast<uintptr_t>(x) & (N * sizeof(T) - 1)) == 0;
 }
 
-// The largest group_top of each group, summed, by the lane whose number the group has (lanes beyond: -infinity); c by expert in `row`.
+// The largest group_top of each group, summed, by the lane whose number the group has (lanes beyond: -infinity); c by expert in `row`.  *size: how
+// large what was summed is, for the bound of its rounding.
 template <class F>
-__device__ __forceinline__ F group_score(const RouteParams& p, const F* row, int lane)
+__device__ __forceinline__ F group_score(const RouteParams& p, const F* row, int lane, F* size)
 {
     F score = (F)-CUDART_INF_F;
+    *size = 0;
     if (lane < p.groups) {
         F best = (F)-CUDART_INF_F, second = (F)-CUDART_INF_F;
         int at = lane % p.per_group;  // lanes begin at different banks
@@ -108,6 +110,7 @@ __device__ __forceinline__ F group_score(const RouteParams& p, const F* row, int
             if (++at == p.per_group) at = 0;
         }
         score = p.group_top == 2 ? best + second : best;
+        *size = (best < -1 || best > 1 ? fabs(best) : 1) + (p.group_top == 2 ? second < -1 || second > 1 ? fabs(second) : 1 : 0);
     }
     return score == score ? score : (F)-CUDART_INF_F;  // -infinity and +infinity
 }
@@ -161,12 +164,14 @@ __device__ __forceinline__ float reciprocal_near(float v)
     return r;
 }
 
-// Which of this lane's experts are in a group that is kept, as bits.  *near: exact sums may keep another one.
+// Which of this lane's experts are in a group that is kept, as bits.  *near: exact sums may keep another one.  margin (negative: the order is exact): as
+// for two c.  A group's sum may be off by half of that for each c in it, relative to max(1, |c|) of that c and not to the sum, in which a bias of
+// 10000 and one of -10000 leave nothing of their size; the constants leave room for the rounding of the sum itself.
 template <int PER>
 __device__ __forceinline__ unsigned open_groups(const RouteParams& p, const float (&c)[PER], int lane, float* row, float margin, bool* near)
 {
     const int first = lane * PER;
-    float score;
+    float score, size;
     bool kept, there;
     unsigned open = 0;
     if (p.group_lanes > 0) {  // a group is that many lanes, a power of two
@@ -183,6 +188,7 @@ __device__ __forceinline__ unsigned open_groups(const RouteParams& p, const floa
         }
         score = p.group_top == 2 ? best + second : best;
         score = score == score ? score : -CUDART_INF_F;  // -infinity and +infinity
+        size = fmaxf(1.0f, fabsf(best)) + (p.group_top == 2 ? fmaxf(1.0f, fabsf(second)) : 0.0f);
         const int mine = lane >> p.log_group_lanes;
         there = mine < p.groups;
         kept = among_best(p, score, mine, [&](int g) { return __shfl_sync(kAllLanes, score, g << p.log_group_lanes); });
@@ -193,7 +199,7 @@ __device__ __forceinline__ unsigned open_groups(const RouteParams& p, const floa
         for (int i = 0; i < PER; ++i)
             if (first + i < p.E) row[first + i] = c[i];
         __syncwarp();
-        score = group_score(p, row, lane);
+        score = group_score(p, row, lane, &size);
         there = lane < p.groups;
         kept = among_best(p, score, lane, [&](int g) { return __shfl_sync(kAllLanes, score, g); });
         const unsigned groups = __ballot_sync(kAllLanes, kept);
@@ -205,8 +211,10 @@ __device__ __forceinline__ unsigned open_groups(const RouteParams& p, const floa
         }
     }
     if (margin >= 0.0f) {
-        const float last = -warp_max(kept ? -score : -CUDART_INF_F), next = warp_max(there && !kept ? score : -CUDART_INF_F);
-        if (next > -CUDART_INF_F && last - next <= margin * fmaxf(1.0f, fabsf(last))) *near = true;
+        // the least that a kept one may be and the most that one left out may be; without a number (infinities of both signs): left out of this
+        const float off = 0.5f * margin * size;
+        const float last = -warp_max(kept ? off - score : -CUDART_INF_F), next = warp_max(there && !kept ? score + off : -CUDART_INF_F);
+        if (next > -CUDART_INF_F && last <= next) *near = true;
     }
     return open;
 }
@@ -285,7 +293,7 @@ __device__ __forceinline__ unsigned choose(const RouteParams& p, const float (&x
     for (int i = 0; i < PER; ++i) c[i] = x[i] > -CUDART_INF_F && c[i] > -CUDART_INF_F ? c[i] : -CUDART_INF_F;  // not available, or NaN
     unsigned open = kAllLanes;
     if (p.top_groups < p.groups) {
-        open = open_groups<PER>(p, c, lane, row, ON_X ? -1.0f : 2.0f * margin, near);
+        open = open_groups<PER>(p, c, lane, row, ON_X ? -1.0f : margin, near);
 #pragma unroll
         for (int i = 0; i < PER; ++i) c[i] = (open >> i) & 1u ? c[i] : -CUDART_INF_F;
     }
@@ -372,7 +380,8 @@ __device__ __forceinline__ unsigned choose_exactly(const RouteParams& p, const T
     }
     __syncwarp();
     if (p.top_groups < p.groups) {
-        const double score = group_score(p, row, lane);
+        double size;
+        const double score = group_score(p, row, lane, &size);
         const unsigned kept = __ballot_sync(kAllLanes, among_best(p, score, lane, [&](int g) { return __shfl_sync(kAllLanes, score, g); }));
         __syncwarp();
 #pragma unroll 1

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from csrspmm_b200 import ops
-from test_gpu_scores import _gen, check_distill, teacher
+from test_gpu_scores import _gen, check_distill, route_f64, teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -158,3 +158,13 @@ def test_distill_from_a_teacher_who_wants_what_is_masked_by_the_lowest(cuda_lib,
     x[3, hit[3, 1]] = -1e38
     check_distill(x, rp, ci, va.flatten(), t, log_probs)
     assert ops.distill_loss(x, rp, ci, va.flatten(), temperature=t, log_probs=log_probs).isfinite().all()
+
+
+@pytest.mark.parametrize("B", [100.0, 30000.0])
+def test_route_between_groups_whose_biases_cancel(cuda_lib, B):
+    """Sums of a large and a small choice are rounded at the size of what they are made of, not of what is left."""
+    x = torch.randn(400_000, 8, device="cuda", generator=_gen(90))
+    bias = torch.tensor([B, -B] * 4, device="cuda") + 0.25 * torch.randn(8, device="cuda", generator=_gen(91))
+    _, ci, _ = ops.route(x, 2, score="sigmoid", bias=bias, groups=4, top_groups=1, group_top=2)
+    want = route_f64(x, 2, bias=bias, score="sigmoid", groups=4, top_groups=1, group_top=2)[0]
+    assert torch.equal(ci.long().view(-1, 2), want)
