@@ -7,10 +7,11 @@
 // there is no counterpart of a choice by rank.
 //
 // One warp owns a row and keeps it in registers, PER consecutive experts a lane, so that a row is read once and the
-// lowest index among equals is the first lane's first element.  The choice has to be the one that exact arithmetic
-// makes: fp32 scores tell two experts apart only where they differ by more than their rounding, so where the last one taken
+// lowest index among equals is the first lane's first element.  The choice has to be the one that scores in 64 bits
+// make: fp32 scores tell two experts apart only where they differ by more than their rounding, so where the last one taken
 // and the first one left out are nearer than that (kSigmoidMargin, kSoftmaxMargin), the warp makes the choice again in 64 bits.
-// Without a bias the order of c is the order of x, and the choice is made on x itself.
+// Without a bias the order of c is the order of x, and the choice is made on x itself, which tells apart what 64 bits round to the same
+// (sigmoids of logits above 37, shares 745 below the largest); sums of two c that rank groups are in 64 bits.
 #pragma once
 
 #include <math_constants.h>
@@ -248,8 +249,8 @@ __device__ __forceinline__ double reciprocal(double v)
     return r;
 }
 
-// The experts a row takes, as bits of the lane that holds them; the choice is made on c in fp32 or, with ON_X, on the logits, whose order is
-// that of c where there is no bias.  *near: in exact arithmetic the choice may be another one.
+// The experts a row takes, as bits of the lane that holds them; the choice is made on c in fp32 or, with ON_X and within groups that are ranked by sums,
+// on the logits, whose order is that of c where there is no bias.  *near: in 64 bits the choice may be another one.
 //
 // Every lane sorts its experts' c; the largest heads of the lanes are taken off until k are, which gives the last c taken, and the experts
 // are those above it and as many at it as are left, in the order of their numbers.  That takes 19 instructions a round where marking
@@ -294,6 +295,12 @@ __device__ __forceinline__ unsigned choose(const RouteParams& p, const float (&x
     unsigned open = kAllLanes;
     if (p.top_groups < p.groups) {
         open = open_groups<PER>(p, c, lane, row, ON_X ? -1.0f : margin, near);
+        if constexpr (!ON_X) {
+            if (p.bias == nullptr) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) c[i] = x[i] > -CUDART_INF_F ? x[i] : -CUDART_INF_F;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) c[i] = (open >> i) & 1u ? c[i] : -CUDART_INF_F;
     }
@@ -318,7 +325,7 @@ __device__ __forceinline__ unsigned choose(const RouteParams& p, const float (&x
     if (last > -CUDART_INF_F) {
         const float next = warp_max(head[0]);  // of those that were not taken off: at `last` itself there may be more
         if constexpr (!ON_X) {
-            if (count > p.k || (next > -CUDART_INF_F && last - next <= margin * fmaxf(1.0f, fabsf(last)))) *near = true;
+            if (p.bias != nullptr && (count > p.k || (next > -CUDART_INF_F && last - next <= margin * fmaxf(1.0f, fabsf(last))))) *near = true;
         }
         if (count == p.k && next < last) {
 #pragma unroll
@@ -387,6 +394,13 @@ __device__ __forceinline__ unsigned choose_exactly(const RouteParams& p, const T
 #pragma unroll 1
         for (int e = lane; e < p.E; e += 32)
             if (!((kept >> (e / p.per_group)) & 1u)) row[e] = CUDART_NAN;
+        if (p.bias == nullptr) {
+#pragma unroll 1
+            for (int e = lane; e < p.E; e += 32) {
+                const float x = to_f32(scores[e]);
+                if (row[e] == row[e]) row[e] = x > -CUDART_INF_F ? (double)x : -CUDART_INF;
+            }
+        }
     }
     unsigned taken = 0;
 #pragma unroll 1

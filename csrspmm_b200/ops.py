@@ -466,11 +466,11 @@ def route(logits: torch.Tensor, k: int, *, bias: torch.Tensor | None = None, sco
 
     Scores are ``softmax`` or ``sigmoid`` of the logits; ``bias`` (E, float32) is added for the choice only.  With
     ``top_groups < groups`` the experts form ``groups`` runs, of which the ``top_groups`` best by the sum of their ``group_top`` (1 or 2)
-    best experts are open to a token.  Ties go to the lower index, and the choice is the one that exact arithmetic makes.  Values are the
-    chosen scores, divided by their sum with ``renormalize``, times ``scale`` (float32).  A logit of -inf is an expert that is not
-    available: it ranks behind all others of the open groups and weighs 0, so that a row with nothing available has k zeros.  A NaN
-    (softmax: or +inf) makes its row's values NaN; the columns stay distinct and inside the matrix.  Experts up to 1024, k and groups
-    up to 32.
+    best experts are open to a token.  Ties go to the lower index, and the choice is the one that scores in 64 bits make; without a bias
+    experts are ranked by their logits, in whose order the scores are.  Values are the chosen scores, divided by their sum with
+    ``renormalize``, times ``scale`` (float32).  A logit of -inf is an expert that is not available: it ranks behind all others of the open
+    groups and weighs 0, so that a row with nothing available has k zeros.  A NaN (softmax: or +inf) makes its row's values NaN; the
+    columns stay distinct and inside the matrix.  Experts up to 1024, k and groups up to 32.
 
     ``values`` is differentiable in ``logits`` (the first derivative; the choice has none, nor has ``bias``).  ``transpose_csr`` of the result lists
     each expert's tokens; ``weighted_spmm`` adds up what the experts answered.

@@ -354,7 +354,8 @@ int csrspmm_b200_transpose(int32_t M, int32_t Kd, int64_t nnz, const int32_t* ro
  * The CSR matrix (T x E) of the k experts that each of T tokens is sent to, from a row of E scores x a token:
  *     s = softmax(x) or sigmoid(x);  c = s + bias (for the choice only; bias may be NULL)
  *     the experts form `groups` runs of E / groups; a group counts as the sum of its group_top (1 or 2) largest c, and the
- *     k largest c of the top_groups best groups are taken (ties: the lower index), as exact arithmetic would
+ *     k largest c of the top_groups best groups are taken (ties: the lower index), with c in 64 bits; without a bias experts are
+ *     ranked by x itself, whose order that of c is
  *     value = scale * s / (sum of the s taken)  with renormalize, else scale * s
  * Rows hold exactly k entries with ascending columns.  An x of -infinity is an expert that is not available: it is
  * ranked behind all others of the groups taken and its value is 0; where nothing is available all k values are 0.  A bias of -infinity or

@@ -168,3 +168,18 @@ def test_route_between_groups_whose_biases_cancel(cuda_lib, B):
     _, ci, _ = ops.route(x, 2, score="sigmoid", bias=bias, groups=4, top_groups=1, group_top=2)
     want = route_f64(x, 2, bias=bias, score="sigmoid", groups=4, top_groups=1, group_top=2)[0]
     assert torch.equal(ci.long().view(-1, 2), want)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_with_groups_ranks_scores_that_round_to_the_same(cuda_lib, score):
+    """Without a bias the order of the scores is that of the logits, where the scores themselves round to 1 or to 0."""
+    high = [40.0, 45.0, 50.0, 41.0] if score == "sigmoid" else [0.0, -800.0, -790.0, -900.0]
+    x = torch.full((3, 8), -50.0 if score == "sigmoid" else -1000.0, device="cuda")
+    x[0, :4] = torch.tensor(high, device="cuda")
+    x[1, 4:] = torch.tensor(high, device="cuda")
+    x[2, :4] = torch.tensor(high[::-1], device="cuda")
+    x[2, 4:] = torch.tensor(high, device="cuda") - 1000.0
+    how = dict(score=score, groups=2, top_groups=1, group_top=2)
+    _, ci, _ = ops.route(x, 2, **how)
+    assert torch.equal(ci.long().view(3, 2), route_f64(x, 2, **how)[0])
+    assert ci.view(3, 2).tolist() == ([[1, 2], [5, 6], [1, 2]] if score == "sigmoid" else [[0, 2], [4, 6], [1, 3]])
