@@ -44,9 +44,14 @@ void first_derivative_only(const char* what)
     if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(what) + " has no second derivative (create_graph)");
 }
 
+void refuse_tangents(std::initializer_list<at::Tensor> tensors, const char* what)
+{
+    for (const at::Tensor& t : tensors) TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), what, " has no forward-mode derivative");
+}
+
 bool wants_gradient(const at::Tensor& t, const char* what)
 {
-    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), what, " has no forward-mode derivative");
+    refuse_tangents({t}, what);
     return at::GradMode::is_enabled() && t.requires_grad();
 }
 
@@ -197,6 +202,7 @@ struct RouteWithGradient : torch::autograd::Function<RouteWithGradient> {
 Triple autograd_route(const at::Tensor& logits, int64_t k, const std::optional<at::Tensor>& bias, c10::string_view score, int64_t groups,
                       int64_t top_groups, int64_t group_top, bool renormalize, double scale)
 {
+    refuse_tangents({logits}, "route");
     const auto out = RouteWithGradient::apply(logits, k, bias, std::string(score), groups, top_groups, group_top, renormalize, scale);
     return {out[0], out[1], out[2]};
 }
@@ -253,6 +259,14 @@ at::Tensor call_sddmm(const at::Tensor& rp, const at::Tensor& ci, const at::Tens
 {
     static const auto op = dispatched<decltype(op_sddmm)>("csrspmm_b200::sddmm");
     return op.call(rp, ci, G, B, alpha);
+}
+
+// No derivative: none is recorded, and a tangent is refused, not dropped.
+at::Tensor autograd_sddmm(const at::Tensor& rp, const at::Tensor& ci, const at::Tensor& G, const at::Tensor& B, double alpha)
+{
+    refuse_tangents({G, B}, "sddmm");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_sddmm(rp, ci, G, B, alpha);
 }
 
 // alpha * A^T * G: in one launch where the matrix is small, else by its transpose
@@ -330,6 +344,7 @@ struct WeightedSpmm : torch::autograd::Function<WeightedSpmm> {
 
 at::Tensor autograd_weighted_spmm(const at::Tensor& rp, const at::Tensor& ci, const at::Tensor& va, const at::Tensor& B, double alpha)
 {
+    refuse_tangents({va, B}, "weighted_spmm");
     return WeightedSpmm::apply(rp, ci, va, B, alpha);
 }
 
@@ -338,8 +353,9 @@ PyObject* py_sddmm(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 {
     BEGIN_BINDING
     expect_args(nargs, 5);
-    return THPVariable_Wrap(op_sddmm(tensor_of(args[0], "row_ptr"), tensor_of(args[1], "col_idx"), tensor_of(args[2], "G"), tensor_of(args[3], "B"),
-                                     as_double(args[4])));
+    const at::Tensor G = tensor_of(args[2], "G"), B = tensor_of(args[3], "B");
+    refuse_tangents({G, B}, "sddmm");
+    return THPVariable_Wrap(op_sddmm(tensor_of(args[0], "row_ptr"), tensor_of(args[1], "col_idx"), G, B, as_double(args[4])));
     END_BINDING
 }
 
@@ -506,7 +522,18 @@ struct DistillWithGradient : torch::autograd::Function<DistillWithGradient> {
 at::Tensor autograd_distill_loss(const at::Tensor& logits, const at::Tensor& rp, const at::Tensor& ci, const at::Tensor& va, double temperature,
                                  bool log_probs)
 {
+    refuse_tangents({logits, va}, "distill_loss");
     return DistillWithGradient::apply(logits, rp, ci, va, temperature, log_probs);
+}
+
+// The gradient is handed out; none is recorded.
+std::tuple<at::Tensor, at::Tensor> autograd_distill_loss_grad(const at::Tensor& logits, const at::Tensor& rp, const at::Tensor& ci, const at::Tensor& va,
+                                                              const at::Tensor& weight, double temperature, bool log_probs)
+{
+    static const auto op = dispatched<decltype(op_distill_loss_grad)>("csrspmm_b200::distill_loss_grad");
+    refuse_tangents({logits, va, weight}, "distill_loss_grad");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(logits, rp, ci, va, weight, temperature, log_probs);
 }
 
 // distill_loss(logits, row_ptr, col_idx, values, temperature, log_probs) -> loss
@@ -527,8 +554,10 @@ PyObject* py_distill_loss_grad(PyObject*, PyObject* const* args, Py_ssize_t narg
 {
     BEGIN_BINDING
     expect_args(nargs, 7);
-    const auto out = op_distill_loss_grad(tensor_of(args[0], "logits"), tensor_of(args[1], "row_ptr"), tensor_of(args[2], "col_idx"),
-                                          tensor_of(args[3], "values"), tensor_of(args[4], "weight"), as_double(args[5]), PyObject_IsTrue(args[6]) == 1);
+    const at::Tensor logits = tensor_of(args[0], "logits"), values = tensor_of(args[3], "values"), weight = tensor_of(args[4], "weight");
+    refuse_tangents({logits, values, weight}, "distill_loss_grad");
+    const auto out = op_distill_loss_grad(logits, tensor_of(args[1], "row_ptr"), tensor_of(args[2], "col_idx"), values, weight, as_double(args[5]),
+                                          PyObject_IsTrue(args[6]) == 1);
     return Py_BuildValue("(NN)", THPVariable_Wrap(std::get<0>(out)), THPVariable_Wrap(std::get<1>(out)));
     END_BINDING
 }
@@ -549,6 +578,8 @@ TORCH_LIBRARY_IMPL(csrspmm_b200, CUDA, scores)
 TORCH_LIBRARY_IMPL(csrspmm_b200, Autograd, scores)
 {
     scores.impl("route", autograd_route);
+    scores.impl("sddmm", autograd_sddmm);
+    scores.impl("distill_loss_grad", autograd_distill_loss_grad);
     scores.impl("weighted_spmm", autograd_weighted_spmm);
     scores.impl("distill_loss", autograd_distill_loss);
 }

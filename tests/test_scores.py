@@ -113,6 +113,23 @@ def test_tangents_are_refused_not_dropped():
                 call()
 
 
+def test_tangents_are_refused_where_no_derivative_is_recorded():
+    import torch.autograd.forward_ad as fwAD
+    O = torch.ops.csrspmm_b200
+    rp, ci, va = torch.zeros(5, dtype=torch.int32), torch.zeros(0, dtype=torch.int32), torch.zeros(0)
+    with fwAD.dual_level():
+        x, w, v = (fwAD.make_dual(torch.zeros(*s), torch.ones(*s)) for s in ((4, 8), (4,), (0,)))
+        flat, one = torch.zeros(4, 8), torch.ones(4)
+        for call in (lambda: ops.sddmm(rp, ci, x, flat), lambda: ops.sddmm(rp, ci, flat, x), lambda: O.sddmm(rp, ci, x, flat, 1.0),
+                     lambda: O.sddmm(rp, ci, flat, x, 1.0), lambda: ops.distill_loss_grad(x, rp, ci, va), lambda: ops.distill_loss_grad(flat, rp, ci, va, w),
+                     lambda: ops.distill_loss_grad(flat, rp, ci, v), lambda: O.distill_loss_grad(x, rp, ci, va, one, 1.0, False),
+                     lambda: O.distill_loss_grad(flat, rp, ci, va, w, 1.0, False), lambda: O.distill_loss_grad(flat, rp, ci, v, one, 1.0, False),
+                     lambda: O.route(x, 2, None, "softmax", 1, 1, 1, True, 1.0), lambda: O.distill_loss(x, rp, ci, va, 1.0, False),
+                     lambda: O.weighted_spmm(rp, ci, v, flat, 1.0)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
 def test_gradients_for_a_teacher_are_refused():
     rp, ci, va = torch.zeros(5, dtype=torch.int32), torch.zeros(0, dtype=torch.int32), torch.zeros(0, requires_grad=True)
     with pytest.raises(RuntimeError, match="no gradient for the teacher"):
