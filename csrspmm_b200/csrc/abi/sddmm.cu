@@ -14,10 +14,14 @@ using namespace csrspmm_b200;
 
 namespace {
 
-// Warps' loads of columns up to which the small product with the transpose is the better way, on the GPU as on the host: 4096 columns of one
-// entry each and 512 columns of G (2^19) 14 us against 20 for transposition and product, a training step 70 against 84; at 2^20 (3000 of 4, 128
-// columns) 33 against 24 on the GPU, 70 against 94 a step.
-constexpr long long kTransposedMost = 1LL << 19;
+// Where the small product with the transpose is the better way: it must not lose where one column holds all entries either, of which the host knows
+// nothing, and its warps must not be more than some waves.  us on the GPU, this kernel and transposition with product (which take 22 from the host,
+// this one 8), entries spread evenly and all in one column:
+//   2048 entries, 64 columns, 512 of G 8 and 19, 19 and 24; 1000 columns, 64 of G 7 and 17, 20 and 19; 4096 entries in one column 35 to 37 and 21 to 34
+//   8192 warps: 1024 entries of 1024 columns, 512 of G 11 and 16, 20 and 22; 2048 of 2048, 64 of G 10 and 15
+//   16384 warps: 512 entries of 4096 columns, 512 of G 14 and 19, 21 and 20; 2048 of 1000, 512 of G 19 and 19, 23 and 25; 32768: 32 and 17
+constexpr long long kTransposedMostEntries = 2048;
+constexpr double kTransposedMostWarps = 1 << 14;
 
 template <int L, int NV, int VW, bool LOOP>
 cudaError_t launch(SddmmParams p, cudaStream_t st)
@@ -72,16 +76,23 @@ extern "C" int csrspmm_b200_sddmm(int32_t M, int32_t Kd, int32_t Nd, int64_t nnz
     return CSRSPMM_B200_OK;
 }
 
-// Warps' worth of columns that the small product with the transpose looks through.
-static long long transposed_work(int32_t Kd, int32_t Nd, int64_t nnz)
+// What the warps of the small product with the transpose divide: groups of rows of C times parts of 32 vectors of `width` floats ...
+static long long transposed_parts(int32_t Kd, int32_t Nd, int width)
 {
-    const long long parts = ((long long)Nd + 32 * kTransposedVectors * 4 - 1) / (32 * kTransposedVectors * 4);
-    return (long long)Kd * parts * ((nnz + 31) / 32);
+    return ((long long)Kd + kTransposedRows - 1) / kTransposedRows * (((long long)Nd / width + 31) / 32);
+}
+// ... each in as many runs of the entries, as a power of two.
+static int log_pieces(int64_t nnz)
+{
+    int n = 0;
+    while (1 << n < kTransposedThreads / 32 && (int64_t)kTransposedRun << n < nnz) ++n;
+    return n;
 }
 
 extern "C" int csrspmm_b200_spmm_transposed_pays(int32_t Kd, int32_t Nd, int64_t nnz)
 {
-    return Kd >= 0 && Nd >= 0 && nnz >= 0 && nnz <= 0x7fffffffLL && transposed_work(Kd, Nd, nnz) <= kTransposedMost;
+    if (Kd < 0 || Nd < 0 || nnz < 0 || nnz > kTransposedMostEntries) return 0;
+    return (double)transposed_parts(Kd, Nd, Nd % 4 == 0 ? 4 : Nd % 2 == 0 ? 2 : 1) * (1 << log_pieces(nnz)) <= kTransposedMostWarps;
 }
 
 extern "C" int csrspmm_b200_spmm_transposed(int32_t M, int32_t Kd, int32_t Nd, int64_t nnz, const int32_t* row_ptr, const int32_t* col_idx,
@@ -99,9 +110,10 @@ extern "C" int csrspmm_b200_spmm_transposed(int32_t M, int32_t Kd, int32_t Nd, i
                ((reinterpret_cast<uintptr_t>(G) | reinterpret_cast<uintptr_t>(C)) & (floats * 4 - 1)) == 0;
     };
     const int width = on(4) ? 4 : on(2) ? 2 : 1;
-    const TransposedParams p = {M, Kd, Nd / width, (int)nnz, row_ptr, col_idx, values, G, ldg, alpha, C, ldc};
-    const long long parts = (p.nvec + 32 * kTransposedVectors - 1) / (32 * kTransposedVectors);
-    const long long ctas = ((long long)Kd * parts + kTransposedThreads / 32 - 1) / (kTransposedThreads / 32);
+    const int pieces = log_pieces(nnz), per_cta = (kTransposedThreads / 32) >> pieces;
+    const int run = (int)((nnz + (32LL << pieces) - 1) / (32LL << pieces)) * 32;
+    const TransposedParams p = {M, Kd, Nd / width, (int)nnz, row_ptr, col_idx, values, G, ldg, alpha, C, ldc, pieces, run};
+    const long long ctas = (transposed_parts(Kd, Nd, width) + per_cta - 1) / per_cta;
     if (ctas > 0x7fffffffLL) {
         set_last_error("spmm_transposed: too many rows and columns");
         return CSRSPMM_B200_ERR_UNSUPPORTED;

@@ -203,12 +203,18 @@ __global__ void __launch_bounds__(kSddmmThreads) sddmm_kernel(SddmmParams p)
 
 // ---- the gradient for B of a small product -----------------------------------------------------------------
 //
-// C = alpha * A^T * G without a transpose: a warp owns a row of C (a column of A) and up to 32 * kTransposedVectors vectors of its columns, looks
-// through all of A's columns and adds up the entries that are its own, in stored order.  That reads nnz columns Kd times, and takes one
-// launch where transposition and product take seven: what a small training step costs is those launches.
+// C = alpha * A^T * G without a transpose: a row of C is a column of A, and whoever owns it looks through A's columns and adds up the entries that are
+// its own.  That reads nnz columns again and again, and takes one launch where transposition and product take seven: what a small training step costs
+// is those launches.
+//
+// 32 vectors of kTransposedRows rows of C belong to `pieces` warps of a CTA, each of which looks through a run of A's entries; the pieces' sums are added
+// in their order.  Runs have kTransposedRun entries as long as there are warps for them, and parts of rows are narrow, so that a column that holds all
+// entries is neither one warp's to walk over nor one SM's to read.  (With a warp for a whole row, and a search and a wait for each entry, such a column
+// took 0.32 us an entry: 640 us for 2048, where transposition and product take 18 to 27.)
 
-constexpr int kTransposedThreads = 256;
-constexpr int kTransposedVectors = 4;
+constexpr int kTransposedThreads = 512;
+constexpr int kTransposedRun = 128;
+constexpr int kTransposedRows = 4;
 
 struct TransposedParams {
     int M, Kd, nvec, nnz;
@@ -220,51 +226,116 @@ struct TransposedParams {
     float alpha;
     float* C;
     long long ldc;
+    int log_pieces, run;  // entries of a piece, a multiple of 32
+};
+
+// A warp's entries among 128, in stored order: the row of G, the value and which of the warp's rows of C
+struct OwnEntries {
+    int row[kTransposedRun];
+    float value[kTransposedRun];
+    int of[kTransposedRun];
 };
 
 template <int VW>
-__global__ void __launch_bounds__(kTransposedThreads) spmm_transposed_kernel(TransposedParams p)
+__global__ void __launch_bounds__(kTransposedThreads, 2) spmm_transposed_kernel(TransposedParams p)
 {
-    constexpr int NV = kTransposedVectors, U = 4;
+    constexpr int U = kTransposedRun / 32, W = kTransposedThreads / 32, R = kTransposedRows, kAtOnce = 4;
+    __shared__ OwnEntries lists[W];
+    __shared__ Vec<VW> sums[W][32];
+    __shared__ bool any[W];
     wait_for_previous_grid();
-    const int lane = threadIdx.x & 31;
-    const long long own = (long long)blockIdx.x * (kTransposedThreads / 32) + (threadIdx.x >> 5);  // row of C and part of its columns
-    const int parts = (p.nvec + 32 * NV - 1) / (32 * NV);
-    const int row = (int)(own / parts), v0 = (int)(own % parts) * 32 * NV + lane;
-    if (row >= p.Kd) return;
-    Vec<VW> sum[NV];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int pieces = 1 << p.log_pieces, piece = warp & (pieces - 1);
+    const long long own = ((long long)blockIdx.x * W + warp) >> p.log_pieces;  // rows of C and part of their columns
+    const int parts = (p.nvec + 31) / 32;
+    const long long row = own / parts * R;
+    const int v = (int)(own % parts) * 32 + lane;
+    const bool there = v < p.nvec;
+    const float* const G = p.G + (long long)v * VW;
+    const long long begin = (long long)piece * p.run, end = row < p.Kd ? min(begin + p.run, (long long)p.nnz) : 0;
+    OwnEntries& list = lists[warp];
+    Vec<VW> sum[R];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) sum[k].zero();
-    for (int base = 0; base < p.nnz; base += 32 * U) {
-        int col[U];
+    for (int k = 0; k < R; ++k) sum[k].zero();
+    bool found = false;
+    for (long long base = begin; base < end; base += 32 * U) {
+        int of[U];
+        unsigned mine[U];
+        int count = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long e = (long long)base + u * 32 + lane;
-            col[u] = e < p.nnz ? min(max(__ldg(p.col_idx + e), 0), p.Kd - 1) : -1;
+            const long long e = base + u * 32 + lane;
+            of[u] = e < end ? (int)min(max(min(max(__ldg(p.col_idx + e), 0), p.Kd - 1) - row, -1LL), (long long)R) : -1;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            unsigned mine = __ballot_sync(kAllLanes, col[u] == row);
-            for (; mine != 0; mine &= mine - 1) {
-                const int e = base + u * 32 + __ffs(mine) - 1;
-                const float* from = p.G + (long long)row_of_entry(p.row_ptr, p.M, e, lane) * p.ldg;
-                const float value = __ldg(p.values + e);
+            mine[u] = __ballot_sync(kAllLanes, of[u] >= 0 && of[u] < R);
+            count += __popc(mine[u]);
+        }
+        if (count == 0) continue;
+        found = true;
+        int r[U] = {};  // the last row that begins at the entry or before it
+        if (count <= 2) {  // all lanes search for one: a step for five of a lane's own
 #pragma unroll
-                for (int k = 0; k < NV; ++k) {
-                    if (v0 + k * 32 < p.nvec) {
-                        Vec<VW> g;
-                        g.load_nc(from + (long long)(v0 + k * 32) * VW);
-                        sum[k].fma(value, g);
-                    }
+            for (int u = 0; u < U; ++u) {
+                for (unsigned left = mine[u]; left != 0; left &= left - 1) {
+                    const int whose = __ffs(left) - 1, at = row_of_entry(p.row_ptr, p.M, (int)(base + u * 32) + whose, lane);
+                    if (lane == whose) r[u] = at;
+                }
+            }
+        } else {
+            for (int length = p.M; length > 1; length -= length / 2) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if ((mine[u] >> lane) & 1u && __ldg(p.row_ptr + r[u] + length / 2) <= (int)(base + u * 32 + lane)) r[u] += length / 2;
+            }
+        }
+        int before = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if ((mine[u] >> lane) & 1u) {
+                const int at = before + __popc(mine[u] & ((1u << lane) - 1u));
+                list.row[at] = r[u];
+                list.value[at] = __ldg(p.values + base + u * 32 + lane);
+                list.of[at] = of[u];
+            }
+            before += __popc(mine[u]);
+        }
+        __syncwarp();
+        for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+            Vec<VW> g[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                if (i0 + i < count && there) g[i].load_nc(G + (long long)list.row[i0 + i] * p.ldg);
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                if (i0 + i < count && there) {
+                    const float value = list.value[i0 + i];
+                    const int k = list.of[i0 + i];
+                    if (k == 0) sum[0].fma(value, g[i]);
+                    else if (k == 1) sum[1].fma(value, g[i]);
+                    else if (k == 2) sum[2].fma(value, g[i]);
+                    else sum[3].fma(value, g[i]);
                 }
             }
         }
-        if (base > INT_MAX - 32 * U) break;
+        __syncwarp();
     }
-    float* const to = p.C + (long long)row * p.ldc;
+    if (lane == 0) any[warp] = found;
+    if (pieces > 1) __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-        if (v0 + k * 32 < p.nvec) sum[k].epilogue0(p.alpha).store(to + (long long)(v0 + k * 32) * VW);
+    for (int k = 0; k < R; ++k) {
+        if (pieces > 1) {
+            if (piece != 0 && found) sums[warp][lane] = sum[k];
+            __syncthreads();
+            if (piece == 0) {
+                for (int q = 1; q < pieces; ++q)
+                    if (any[warp + q]) sum[k].fma(1.0f, sums[warp + q][lane]);
+            }
+            __syncthreads();
+        }
+        if (piece == 0 && row + k < p.Kd && there) sum[k].epilogue0(p.alpha).store(p.C + (row + k) * p.ldc + (long long)v * VW);
+    }
 }
 
 }  // namespace csrspmm_b200

@@ -278,7 +278,10 @@ at::Tensor op_spmm_transposed(const at::Tensor& rp, const at::Tensor& ci, const 
         want(va.size(0) == ci.size(0), "values and col_idx differ in length");
         want(G.size(0) == rp.size(0) - 1, "G must have a row for each row of the matrix");
         const int32_t Nd = as_int32(G.size(1), "G has too many columns"), M = as_int32(G.size(0), "too many rows");
-        if (!g_scores.transposed_pays(as_int32(Kd, "too many columns"), Nd, ci.size(0))) {
+        // an odd number of columns is counted in single floats, as those of an unaligned G are read
+        const bool whole = Nd % 4 == 0 ? reinterpret_cast<uintptr_t>(G.data_ptr()) % 16 == 0 && leading(G) % 4 == 0
+                                       : reinterpret_cast<uintptr_t>(G.data_ptr()) % 8 == 0 && leading(G) % 2 == 0;
+        if (!g_scores.transposed_pays(as_int32(Kd, "too many columns"), whole ? Nd : Nd | 1, ci.size(0))) {
             Product q;
             std::tie(q.rp, q.ci, q.va) = transpose(rp, ci, va, Kd);
             q.B = G;

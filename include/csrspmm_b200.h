@@ -395,9 +395,9 @@ int csrspmm_b200_route_backward(const csrspmm_b200_route_args* args, const int32
 int csrspmm_b200_sddmm(int32_t M, int32_t Kd, int32_t Nd, int64_t nnz, const int32_t* row_ptr, const int32_t* col_idx, const float* G,
                        int64_t ldg, const float* B, int64_t ldb, float alpha, float* out, csrspmm_b200_stream_t stream);
 
-/* C = alpha * A^T * G (Kd x Nd, every element written) for a small A, in one launch and without its transpose: every row of C looks through all of
- * A's columns, so that the time grows with Kd * nnz; _pays says whether that is the better way than csrspmm_b200_transpose and a product.
- * Sums are in stored order.  Device pointers, asynchronous. */
+/* C = alpha * A^T * G (Kd x Nd, every element written) for a small A, in one launch and without its transpose: rows of C look through all of A's
+ * columns, so that the time grows with Kd * nnz; _pays says whether that is the better way than csrspmm_b200_transpose and a product, wherever the
+ * entries are.  Sums are taken in a fixed order.  Device pointers, asynchronous. */
 int csrspmm_b200_spmm_transposed_pays(int32_t Kd, int32_t Nd, int64_t nnz);
 int csrspmm_b200_spmm_transposed(int32_t M, int32_t Kd, int32_t Nd, int64_t nnz, const int32_t* row_ptr, const int32_t* col_idx, const float* values,
                                  const float* G, int64_t ldg, float alpha, float* C, int64_t ldc, csrspmm_b200_stream_t stream);

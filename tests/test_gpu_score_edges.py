@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from csrspmm_b200 import ops
-from test_gpu_scores import _gen, check_distill, route_f64, teacher
+from test_gpu_scores import U, _gen, _rows, check_distill, route_f64, teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +183,29 @@ def test_route_with_groups_ranks_scores_that_round_to_the_same(cuda_lib, score):
     _, ci, _ = ops.route(x, 2, **how)
     assert torch.equal(ci.long().view(3, 2), route_f64(x, 2, **how)[0])
     assert ci.view(3, 2).tolist() == ([[1, 2], [5, 6], [1, 2]] if score == "sigmoid" else [[0, 2], [4, 6], [1, 3]])
+
+
+@pytest.mark.parametrize("Nd", [1, 6, 64, 513])
+@pytest.mark.parametrize("Kd", [1, 3, 5, 70, 1000])
+@pytest.mark.parametrize("nnz,kind", [(1, "one"), (31, "one"), (129, "spread"), (700, "one"), (700, "two"), (2048, "one"), (2048, "spread"), (5000, "two"), (40_000, "one")])
+def test_small_product_with_the_transpose_of_crowded_columns(cuda_lib, nnz, kind, Kd, Nd):
+    """All entries in one column, in two, and spread; and more of them than the operator takes this way for."""
+    import ctypes as C
+    from csrspmm_b200 import _lib
+    M = max(1, nnz // 3)
+    rp = torch.zeros(M + 1, dtype=torch.int32, device="cuda")
+    rp[1:] = torch.randint(0, nnz + 1, (M,), device="cuda", generator=_gen(nnz)).sort().values
+    rp[M] = nnz
+    column = {"one": [Kd - 1], "two": [0, Kd // 2], "spread": list(range(Kd))}[kind]
+    ci = torch.tensor(column, device="cuda", dtype=torch.int32)[torch.randint(0, len(column), (nnz,), device="cuda", generator=_gen(2))]
+    va, G = torch.randn(nnz, device="cuda", generator=_gen(3)), torch.randn(M, Nd, device="cuda", generator=_gen(4))
+    terms = va.double()[:, None] * G.double()[_rows(rp)]
+    want, size = (torch.zeros(Kd, Nd, dtype=torch.float64, device="cuda").index_add(0, ci.long(), t) for t in (terms, terms.abs()))
+    bound = (int(torch.bincount(ci.long()).max()) + 17) * U * 1.5 * size + 1e-38  # a sum in turn, of runs or of all, and the factor
+    out = torch.full((Kd + 1, Nd + 3), 7.0, device="cuda")
+    assert _lib.lib().csrspmm_b200_spmm_transposed(M, Kd, Nd, nnz, rp.data_ptr(), ci.data_ptr(), va.data_ptr(), G.data_ptr(), Nd, 1.5, out.data_ptr(),
+                                                   Nd + 3, C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    assert ((out[:Kd, :Nd].double() - 1.5 * want).abs() <= bound).all() and (out[:Kd, Nd:] == 7).all() and (out[Kd] == 7).all()
+    again = torch.ops.csrspmm_b200.spmm_transposed(rp, ci, va, G, Kd, 1.5)
+    assert ((again.double() - 1.5 * want).abs() <= bound).all()
+    assert torch.equal(again, torch.ops.csrspmm_b200.spmm_transposed(rp, ci, va, G, Kd, 1.5))

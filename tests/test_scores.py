@@ -81,6 +81,15 @@ def test_bad_arguments_of_the_small_product_with_the_transpose_are_refused():
     assert L.csrspmm_b200_spmm_transposed_pays(-1, 64, 500) == 0
 
 
+def test_the_small_product_with_the_transpose_is_taken_only_where_no_column_can_be_crowded():
+    pays = _lib.lib().csrspmm_b200_spmm_transposed_pays
+    for Kd, Nd, nnz in ((64, 512, 131_072), (32, 512, 524_288), (64, 512, 262_144), (1, 512, 1 << 24), (1, 1, 1 << 24), (8, 64, 32_768), (200, 64, 2049),
+                        (2048, 512, 2048), (1024, 513, 1024), (1 << 30, 1 << 30, 2048), (2 ** 31 - 1, 2 ** 31 - 1, 1)):
+        assert pays(Kd, Nd, nnz) == 0, (Kd, Nd, nnz)
+    for Kd, Nd, nnz in ((1, 1, 0), (8, 512, 2048), (64, 512, 2048), (1024, 512, 1024), (512, 2048, 512), (2048, 64, 2048), (256, 513, 512)):
+        assert pays(Kd, Nd, nnz) == 1, (Kd, Nd, nnz)
+
+
 def test_bad_pointers_of_the_sampled_product_are_refused():
     good = [4, 4, 4, 5, P, P, P, 4, P, 4, 1.0, P, None]
     for at, value in ((4, None), (5, None), (6, None), (7, 3), (8, None), (9, 3), (11, None)):
