@@ -209,3 +209,13 @@ def test_small_product_with_the_transpose_of_crowded_columns(cuda_lib, nnz, kind
     again = torch.ops.csrspmm_b200.spmm_transposed(rp, ci, va, G, Kd, 1.5)
     assert ((again.double() - 1.5 * want).abs() <= bound).all()
     assert torch.equal(again, torch.ops.csrspmm_b200.spmm_transposed(rp, ci, va, G, Kd, 1.5))
+
+
+def test_the_64_bit_exponential_and_reciprocal_of_the_choice(cuda_lib):
+    """Over their whole range, against long double; the program states the bounds."""
+    import subprocess
+    from pathlib import Path
+    exe = Path(__file__).parent / "cpp" / "_bin" / "test_route_math"
+    assert exe.exists(), "tests/cpp/_bin/test_route_math not built (python -m csrspmm_b200.build)"
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0, run.stdout + run.stderr
