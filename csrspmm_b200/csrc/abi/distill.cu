@@ -29,6 +29,7 @@ int check(const csrspmm_b200_distill_args* a)
     if (a->logit_type < CSRSPMM_B200_F32 || a->logit_type > CSRSPMM_B200_BF16) return refuse("unknown logit_type");
     if (!(a->temperature > 0.0f) || !std::isfinite(a->temperature) || !std::isfinite(1.0f / a->temperature))
         return refuse("temperature has to be positive and finite, its inverse too");
+    if (!std::isnormal(a->temperature * a->temperature)) return refuse("the square of the temperature has to be in fp32");
     if (a->V == 0 && a->nnz > 0) return refuse("entries, but no columns");
     if (a->T > 0 && (a->row_ptr == nullptr || (a->V > 0 && a->logits == nullptr) || (a->nnz > 0 && (a->col_idx == nullptr || a->values == nullptr))))
         return refuse("null pointer");

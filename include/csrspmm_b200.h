@@ -420,7 +420,7 @@ typedef struct csrspmm_b200_distill_args {
     const int32_t* row_ptr;
     const int32_t* col_idx;
     const float* values;
-    float temperature;    /* t: positive and finite */
+    float temperature;    /* t: positive and finite, 1 / t and t^2 too */
     int32_t log_probs;
 } csrspmm_b200_distill_args;
 /* loss: T floats.  stats (16-byte aligned, 4 * T floats): what _distill_backward needs, or NULL.  Asynchronous. */

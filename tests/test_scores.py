@@ -48,6 +48,16 @@ def test_bad_distillation_is_refused_before_any_cuda_call(change):
     assert L.csrspmm_b200_distill_grad(C.byref(a), P, 1, P, P, 100, None) == _lib.ERR_BAD_ARG
 
 
+@pytest.mark.parametrize("t", [1e20, 2e19, 1e-20, 1e-37])
+def test_temperatures_whose_square_is_not_in_fp32_are_refused(t):
+    """The loss is t^2 times what is left of sums of numbers of size 1."""
+    L, a = _lib.lib(), _distill(temperature=t)
+    assert L.csrspmm_b200_distill(C.byref(a), P, P, None) == _lib.ERR_BAD_ARG
+    assert b"square of the temperature" in L.csrspmm_b200_last_error()
+    assert L.csrspmm_b200_distill_backward(C.byref(a), P, P, 1, P, 100, None) == _lib.ERR_BAD_ARG
+    assert L.csrspmm_b200_distill_grad(C.byref(a), P, 1, P, P, 100, None) == _lib.ERR_BAD_ARG
+
+
 def test_missing_outputs_are_refused():
     L, r, d = _lib.lib(), _route(), _distill()
     bad = _lib.ERR_BAD_ARG
