@@ -93,9 +93,9 @@ constexpr int kDynamicSmem = 216 * 1024;  // of a CTA, beside RingShared
 // and 304, 328, 471 us, of 9000 282, 747, 1947 and 355, 374, 545, 4096 of 30000 124, 316, 752 and 149, 152, 202, 2048 of 131072 270, 640, 1481
 // and 355, 360, 443, 64 of 131072 15, 24, 51 and 19, 20, 25.  With 32 the ring takes 0.4 to 0.65 of the other's time, but for 128 of 600000 (115 and 92).
 constexpr int kMostEntries = kListed;
-// And where one row may hold so many that its manager's walks over them (eight, each up to 25 cycles an entry) come near the limit of the waits for
-// it, 2^28 attempts of 20 cycles and more.
-constexpr long long kMostWalked = 1LL << 24;
+// And where one row may hold so many that its manager's walks over them (four before the workers go on, each up to 20 cycles an entry: 2.7e9 cycles)
+// come near the limit of the waits for it, 2^28 attempts of 20 cycles and more.
+constexpr long long kMostWalked = 1LL << 25;
 
 template <class T, int WORKERS, bool GRADIENT>
 cudaError_t launch_ring(const csrspmm_b200_distill_args* a, DistillParams p, int ctas_per_sm, cudaStream_t st)

@@ -244,7 +244,7 @@ def test_a_failed_launch_is_reported(fake):
 
 
 def test_batches_in_which_a_row_may_hold_very_many_entries_take_the_kernel_without_waits(fake):
-    for nnz, ring in ((1 << 24, True), ((1 << 24) + 1, False)):
+    for nnz, ring in ((1 << 25, True), ((1 << 25) + 1, False)):
         a = _distill(T=200_000, V=100_000, ld=100_000, nnz=nnz)
         for call in (lambda: fake.csrspmm_b200_distill(C.byref(a), P, P, None), lambda: fake.csrspmm_b200_distill_grad(C.byref(a), P, 1, P, P, 100_000, None)):
             fake.fake_reset(0)
